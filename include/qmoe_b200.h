@@ -266,6 +266,40 @@ int dq_gemv_nvfp4_bf16(const uint8_t *w, const uint8_t *sc, const float *s2, con
 int dq_dequant_rows(int fmt, const uint8_t *w, const uint8_t *sc, const float *s, int64_t N, int64_t K, int64_t r0,
                     int64_t r1, void *out, int out_dtype, void *stream);
 
+/* ------------------------------------------------------------------ four-bit activations */
+
+/* No counterpart kernel in the reference (its checkpoints arrive quantized). x [M, K] in x_dtype, rows ldx elements
+ * apart (ldx >= K) -> NVFP4: codes w [M, K/2] u8, scales sc [M, K/16] e4m3, s f32: one per row ([M], per_row != 0) or
+ * one for the tensor ([1]). s is the smallest power of two >= 2^-126 with amax <= 6*448*s; sc the nearest e4m3 of
+ * amax16 / (6 s), codes the nearest e2m1 of x / (s sc), ties to even, decided exactly. A block that holds an infinity
+ * or a NaN gets the scale NaN; s ignores those elements. atoms (NULL: none): the same scales in the layout
+ * dq_gemm_nvfp4 reads, ceil(M/128) * ceil(K/64) * 512 bytes; bytes of rows past M are left as they are. K a multiple
+ * of 16; w 8-byte aligned. */
+int dq_quantize_nvfp4(const void *x, int x_dtype, int64_t ldx, int64_t M, int64_t K, int per_row, uint8_t *w, uint8_t *sc,
+                      float *s, uint8_t *atoms, void *stream);
+
+/* sc [N, K/16] -> atoms: the layout of block scales that dq_gemm_nvfp4 reads. 512-byte atoms of 128 rows x 4 scales,
+ * [ceil(N/128)][ceil(K/64)]; inside an atom the four scales of row r lie at (r % 32) * 16 + (r % 128 / 32) * 4. */
+int dq_scale_atoms(const uint8_t *sc, int64_t N, int64_t K, uint8_t *atoms, void *stream);
+
+/* dq_dequant_rows for NVFP4 with one s ([1]) or one per row (s_per_row != 0, s [N]); w 8-byte aligned. */
+int dq_dequant_nvfp4(const uint8_t *w, const uint8_t *sc, const float *s, int s_per_row, int64_t N, int64_t K, int64_t r0,
+                     int64_t r1, void *out, int out_dtype, void *stream);
+
+/* No counterpart in the reference (its products of more than two rows dequantize to bf16 and call F.linear).
+ * y[m, n] = sx[m] * sw[n] * sum_k (q_x sc_x)[m, k] * (q_w sc_w)[n, k], NVFP4 activations x [M, K/2] times NVFP4
+ * weights w [N, K/2], both scales as atoms, accumulated in fp32; sw, sx one value or one per row. y [M, N] in y_dtype,
+ * rounded once and then as dq_gemv_nvfp4_bf16's epilogues: 0 the product, 1 relu^2 of it, 2 the sum with residual
+ * [M, N] (of y_dtype). Block scales are non-negative (the sign bit is not read). Any M, N >= 1; K a multiple of 32;
+ * codes and atoms 16-byte aligned. Sums run in a fixed
+ * order: the same call gives the same bits. A device-side wait that runs out (qmoe_set_wait_cycles) records QMOE_ERR_TIMEOUT, read by dq_gemm_nvfp4_status. */
+int dq_gemm_nvfp4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int sw_per_row, const uint8_t *x,
+                  const uint8_t *x_atoms, const float *sx, int sx_per_row, int M, int N, int K, int epilogue,
+                  const void *residual, void *y, int y_dtype, void *stream);
+
+/* The first error the calls of dq_gemm_nvfp4 on the current device recorded since the last clear; waits for stream. */
+int dq_gemm_nvfp4_status(int clear, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -50,6 +50,11 @@ SIGNATURES = {
     "qmoe_block_deq": (_i, [_p, _f, _f, _p, _p, _p]),
     "dq_gemv_fp8": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _p]),
     "dq_gemv_nvfp4": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _p]),
+    "dq_quantize_nvfp4": (_i, [_p, _i, _i64, _i64, _i64, _i, _p, _p, _p, _p, _p]),
+    "dq_scale_atoms": (_i, [_p, _i64, _i64, _p, _p]),
+    "dq_dequant_nvfp4": (_i, [_p, _p, _p, _i, _i64, _i64, _i64, _i64, _p, _i, _p]),
+    "dq_gemm_nvfp4": (_i, [_p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i, _p]),
+    "dq_gemm_nvfp4_status": (_i, [_i, _p]),
     "dq_dequant_rows": (_i, [_i, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i, _p]),
 }
 

@@ -182,6 +182,8 @@ int dq_dequant_rows(int fmt, const uint8_t *w, const uint8_t *sc, const float *s
     if (!w || !s || !out || (fmt == 1 && !sc)) return QMOE_ERR_NULL;
     if ((fmt != 0 && fmt != 1) || K < 16 || (K % 16) || r0 < 0 || r1 < r0 || r1 > N) return QMOE_ERR_SHAPE;
     if (!valid_dtype(out_dtype)) return QMOE_ERR_DTYPE;
+    if (fmt == 1 && !(reinterpret_cast<uintptr_t>(w) & 7u) && K <= (1 << 24))   // whole 16-element blocks at once
+        return dq_dequant_nvfp4(w, sc, s, 0, N, K, r0, r1, out, out_dtype, stream);
     if (int e = current_device(nullptr, nullptr)) return e;
     if (r1 == r0) return QMOE_OK;
     const int64_t total = (r1 - r0) * (fmt == 0 ? K : K / 2);

@@ -74,6 +74,9 @@ inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3
 
 inline bool valid_dtype(int dt) { return dt == QMOE_DT_F32 || dt == QMOE_DT_BF16 || dt == QMOE_DT_F16; }
 
+// Bound on each device-side wait of the tensor-core kernels on device `dev`, in SM cycles (qmoe_set_wait_cycles).
+long long wait_cycles(int dev);
+
 inline cudaStream_t as_stream(void *s) { return reinterpret_cast<cudaStream_t>(s); }
 
 } // namespace qmoe

@@ -18,10 +18,9 @@
 //   5. pf_hplanes: h in its tile's frame as three NVFP4 planes.
 //   6. pfb_gemm<DOWN>: per (tile, 128 output rows), K = 2688; epilogue y = D * 2^(4 - S0) * s2d * coef.
 //   7. pf_combine: out[t] = sum_k Op[pos(t, k)] in k order (deterministic, as nem_super.py:309-347).
-#include <cuda.h>
-
 #include "common.cuh"
 #include "host.h"
+#include "tc.cuh"
 
 namespace qmoe {
 namespace pf {
@@ -238,95 +237,6 @@ __global__ void __launch_bounds__(256) pf_combine_kernel(const Params p) {
         acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
     reinterpret_cast<float4 *>(p.out + (int64_t)t * LAT)[threadIdx.x] = acc;
-}
-
-// ------------------------------------------------------------------------------------------ tcgen05
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-__device__ __forceinline__ void named_sync(int id, int threads) {
-    asm volatile("barrier.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
-// Shared-memory matrix descriptor (tcgen05 "matrix descriptor", version 1): start, leading and stride
-// byte offsets in 16-byte units, layout type in bits 61-63 (0 = no swizzle, 2 = 128-byte swizzle).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo, uint32_t layout) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-           ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | ((uint64_t)layout << 61);
-}
-
-// Arrives on `bar` once every tcgen05.mma this thread issued before has completed.
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-
-// 32 lanes x 32 consecutive f32 columns of tensor memory -> 32 registers per thread.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-}
-
-// 3-D tiled TMA load (box {x, y, 1}) into this CTA's shared memory, completing on `bar`.
-// 1-D bulk copy global -> shared (16-byte aligned addresses, size a multiple of 16), completing on bar.
-__device__ __forceinline__ void bulk_g2s_nohint(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_u32(dst)),
-                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-
-__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-            "r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
-}
-
-// 32 lanes x 16 consecutive f32 columns of tensor memory -> 16 registers per thread.
-// 16 consecutive 32-bit columns of this warp's 32 TMEM lanes from registers (thread i -> lane base + i).
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-
-
-// Bounded wait for the phase with the given parity: false after `limit` SM clock cycles.
-__device__ __forceinline__ bool mbar_wait_for(uint64_t *bar, uint32_t parity, long long limit) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-        if (clock64() - t0 > limit) return false;
-    }
-    return true;
-}
-
-__device__ __forceinline__ bool lane_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status,
-                                          long long limit) {
-    if (mbar_try_wait(bar, parity)) return true;   // ready: no need to look at the abort flag
-    const bool ok = !*abort_flag && mbar_wait_for(bar, parity, limit);
-    if (!ok) {
-        set_error(status, DEV_ERR_TIMEOUT);
-        *abort_flag = 1;
-    }
-    return ok;
 }
 
 // ------------------------------------------------------------------------------------------ block-scaled
@@ -572,21 +482,6 @@ __global__ void __launch_bounds__(256) pf_hplanes_kernel(const Params p) {
     }
 }
 
-__device__ __forceinline__ void mma_nvfp4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc,
-                                          uint32_t tsfa, uint32_t tsfb) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.block16 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(tsfa), "r"(tsfb)
-        : "memory");
-}
-
-// Instruction descriptor of kind::mxf4nvf4: A, B e2m1 (format 1), K-major, e4m3 scales, M = 128, N = n, K = 64.
-__device__ __forceinline__ uint32_t instr_desc_nvfp4(int n) {
-    return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-}
-
 // The grouped GEMM on block-scaled NVFP4 MMA; persistent: one CTA per SM walks the items (tile, 128 weight
 // rows) i = blockIdx.x, blockIdx.x + gridDim.x, ... (consecutive items share a tile, whose planes stay in L2).
 // Roles: warps 4..5 load the weight stages (TMA, 8 KB, 64-byte swizzle); warps 6..7 the NP activation planes
@@ -594,36 +489,6 @@ __device__ __forceinline__ uint32_t instr_desc_nvfp4(int n) {
 // laid out by the plane kernels); warp 8 bulk-copies the item's 128 weight-scale rows into a slab and
 // rearranges each stage's two weight atoms from it; warps 10..13 store the stage's atoms into its TMEM scale
 // slot; warp 9 issues the MMAs into one of two TMEM accumulators while warps 0..3 drain the other (epilogue).
-// Waits of the producer and epilogue roles: between polls the thread sleeps, so that polling warps leave the
-// issue slots of their SM sub-partition to the MMA-issuing warp.
-__device__ __forceinline__ bool mbar_wait_bo(uint64_t *bar, uint32_t parity, long long limit) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-        __nanosleep(200);
-        if (clock64() - t0 > limit) return false;
-    }
-    return true;
-}
-
-__device__ __forceinline__ bool lane_wait_bo(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status,
-                                             long long limit) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const bool ok = !*abort_flag && mbar_wait_bo(bar, parity, limit);
-    if (!ok) {
-        set_error(status, DEV_ERR_TIMEOUT);
-        *abort_flag = 1;
-    }
-    return ok;
-}
-
-__device__ __forceinline__ bool warp_wait_bo(uint64_t *bar, uint32_t parity, int lane, volatile int *abort_flag,
-                                             int *status, long long limit) {
-    bool ok = true;
-    if (lane == 0) ok = lane_wait_bo(bar, parity, abort_flag, status, limit);
-    return __shfl_sync(0xffffffffu, ok, 0);
-}
-
 template <int PH>
 __global__ void __launch_bounds__(BS_THREADS, 1)
     pfb_gemm_kernel(const Params p, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ PlaneMaps tm_b) {
@@ -1236,23 +1101,6 @@ inline WsLayout ws_layout(int T, int topk, int ne, bool layout_T) {
     return L;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-inline EncodeTiledFn encode_tiled() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(f);
-    });
-    return fn;
-}
-
 // The store as a u8 tensor [ne][BLOCK / pitch][pitch] (expert stride bstride), for TMA boxes of
 // {box_x bytes, box_y rows} out of one block region.
 inline bool make_store_map(CUtensorMap *m, const void *store, int64_t bstride, int ne, int pitch, int box_x,
@@ -1285,6 +1133,12 @@ std::atomic<uint64_t> g_smem_up{0}, g_smem_dn_o{0};
 std::atomic<long long> g_wait_cycles[MAX_DEVICES];   // 0: the default bound
 
 } // namespace pf
+
+long long wait_cycles(int dev) {
+    const long long wc = pf::g_wait_cycles[dev].load(std::memory_order_relaxed);
+    return wc > 0 ? wc : WAIT_CYCLES;
+}
+
 } // namespace qmoe
 
 using namespace qmoe;
@@ -1331,8 +1185,7 @@ int qmoe_prefill_grouped(const uint8_t *store, int64_t block_stride, int n_exper
     p.tiles_cap = L.tiles_cap;
     p.out = out;
     p.status = reinterpret_cast<int *>(ws + L.status);
-    const long long wc = g_wait_cycles[dev].load(std::memory_order_relaxed);
-    p.wait_cycles = wc > 0 ? wc : WAIT_CYCLES;
+    p.wait_cycles = wait_cycles(dev);
     p.tile_count = reinterpret_cast<int *>(ws + L.tile_count);
     p.cnt = reinterpret_cast<int *>(ws + L.cnt);
     p.eoff = reinterpret_cast<int *>(ws + L.eoff);

@@ -6,6 +6,11 @@ Same quantized-weight dict {"fmt", "w", "sc", "s", "N", "K"} (dense_q.py:237-247
 Dispatch (dense_q.py:215-234): M == 1 -> gemv; 2 <= M <= MB_MAX -> gemv_mb (weights read once for all
 vectors; the reference's limit is 2, these kernels take up to 4); larger M -> exact dequantization to
 bf16 in row chunks (dq_dequant_rows) + F.linear (cuBLAS), as the reference does.
+
+Four-bit activations: `quantize` makes the same dict from a tensor, with one scale ("nvfp4", a weight) or one per row
+("nvfp4_rows", activations: a row's result does not depend on the other rows); `gemm` multiplies two of them on the
+tensor cores, and `qlinear_a4` is both, a linear that quantizes its input. `prepare` lays a loaded weight's scales
+out for `gemm` once. These are inference operators: they refuse inputs that need a gradient.
 """
 import types
 
@@ -26,6 +31,8 @@ E2M1_T = None
 
 def _gemv(q, x2, M):
     N, K = q["N"], q["K"]
+    if q["fmt"] == "nvfp4_rows":
+        raise C.QmoeError("the GEMVs take one scale per weight; this one has a scale per row (use gemm)")
     x2 = x2.contiguous()
     out = torch.empty(M, N, dtype=torch.float32, device=x2.device)
     st = C.stream_of(x2)
@@ -65,6 +72,11 @@ def dequant_rows(q, r0, r1, out):
     if not out.is_contiguous():
         raise C.QmoeError("out must be contiguous")
     sc = q.get("sc")
+    if q["fmt"] == "nvfp4_rows":
+        with _on(out):
+            C.call("dq_dequant_nvfp4", C.ptr(q["w"]), C.ptr(sc), C.ptr(q["s"]), 1, q["N"], q["K"], r0, r1, C.ptr(out),
+                   C.dtype_code(out), C.stream_of(out))
+        return out
     C.call("dq_dequant_rows", 0 if q["fmt"] == "fp8" else 1, C.ptr(q["w"]), C.ptr(sc) if sc is not None else None,
            C.ptr(q["s"]), q["N"], q["K"], r0, r1, C.ptr(out), C.dtype_code(out), C.stream_of(out))
     return out
@@ -123,6 +135,134 @@ def attach(lin, q):
     lin._q = q
     object.__setattr__(lin, "weight", q["w"])
     lin.forward = types.MethodType(_fwd, lin)
+
+
+class _on:
+    """The tensor's device as the current one, for the launch (nothing to do where it is)."""
+
+    def __init__(self, t):
+        self.dev = t.device.index if t.is_cuda else None
+
+    def __enter__(self):
+        self.was = torch.cuda.current_device() if self.dev is not None else None
+        if self.was != self.dev:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *a):
+        if self.was != self.dev:
+            torch.cuda.set_device(self.was)
+
+
+def _atoms_bytes(rows, K):
+    return (rows + 127) // 128 * ((K + 63) // 64) * 512
+
+
+def _no_grad(*ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise C.QmoeError("the four-bit operators have no gradient: call them under torch.no_grad()")
+
+
+def quantize(x, per_row=True):
+    """x [M, K] (bf16, fp16 or fp32; K a multiple of 16; rows may be strided) -> quantized dict: codes "w" [M, K/2],
+    block scales "sc" [M, K/16] (e4m3 bytes), "s" f32 [M] with fmt "nvfp4_rows" (per_row), or [1] with fmt "nvfp4"
+    (one scale for the tensor: a weight of this module), and "sca", the scales as gemm reads them. s is the smallest
+    power of two with amax <= 2688 s, scales and codes the nearest, ties to even. A 16-element block that holds an
+    infinity or a NaN reads back as NaN; the others are as if that value were zero."""
+    _no_grad(x)
+    if x.dim() != 2:
+        raise C.QmoeError("quantize takes a matrix [M, K]")
+    M, K = x.shape
+    if K < 16 or K % 16:
+        raise C.QmoeError(f"quantize takes rows of a positive multiple of 16 elements (got {K})")
+    if M == 0 and not per_row:
+        raise C.QmoeError("a tensor without rows has no scale")
+    C.ptr(x)
+    dt = C.dtype_code(x)
+    if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
+        x = x.contiguous()
+    dev = x.device
+    q = {"fmt": "nvfp4_rows" if per_row else "nvfp4", "w": torch.empty(M, K // 2, dtype=torch.uint8, device=dev),
+         "sc": torch.empty(M, K // 16, dtype=torch.uint8, device=dev),
+         "s": torch.empty(M if per_row else 1, dtype=torch.float32, device=dev), "N": M, "K": K,
+         "sca": torch.empty(_atoms_bytes(M, K), dtype=torch.uint8, device=dev)}
+    if M:
+        with _on(x):
+            C.call("dq_quantize_nvfp4", C.ptr(x), dt, int(x.stride(0)) if M > 1 else K, M, K, int(per_row),
+                   C.ptr(q["w"]), C.ptr(q["sc"]), C.ptr(q["s"]), C.ptr(q["sca"]), C.stream_of(x))
+    return q
+
+
+def prepare(q):
+    """A weight ready for gemm: the dict with "sca", its block scales as the tensor cores read them, added (the
+    other tensors are shared with q)."""
+    if q["fmt"] not in ("nvfp4", "nvfp4_rows"):
+        raise C.QmoeError(f"gemm takes NVFP4 weights (got {q['fmt']})")
+    if "sca" in q:
+        return q
+    N, K = q["N"], q["K"]
+    sc = q["sc"].contiguous()
+    sca = torch.empty(_atoms_bytes(N, K), dtype=torch.uint8, device=sc.device)
+    with _on(sc):
+        C.call("dq_scale_atoms", C.ptr(sc), N, K, C.ptr(sca), C.stream_of(sc))
+    return {**q, "sca": sca}
+
+
+_ACTS = {None: 0, "relu2": 1}
+
+
+def gemm(q, xq, dtype=torch.bfloat16, act=None, residual=None):
+    """y [M, N] in dtype = dequant(xq) @ dequant(q).T for two NVFP4 dicts (xq of quantize: activations; q: a weight,
+    best one that went through prepare, else its scales are laid out in this call), products exact, fp32 sums in a
+    fixed order. act "relu2": relu(y)^2; residual [M, N] in dtype: y + residual; each on y rounded to dtype, as the
+    unfused torch operators. K a multiple of 32; rows without elements are refused."""
+    for d in (q, xq):
+        if d["fmt"] not in ("nvfp4", "nvfp4_rows"):
+            raise C.QmoeError(f"gemm takes NVFP4 operands (got {d['fmt']})")
+    M, N, K = xq["N"], q["N"], q["K"]
+    if xq["K"] != K:
+        raise C.QmoeError(f"gemm: {xq['K']} elements per activation row, {K} per weight row")
+    if K % 32:
+        raise C.QmoeError(f"gemm takes rows of a multiple of 32 elements (got {K})")
+    if act not in _ACTS or (act is not None and residual is not None):
+        raise C.QmoeError("gemm: act is None or 'relu2', and not together with a residual")
+    if dtype not in C.DT:
+        raise C.QmoeError(f"unsupported output dtype {dtype}")
+    dev = xq["w"].device
+    if q["w"].device != dev:
+        raise C.QmoeError(f"gemm: weight on {q['w'].device}, activations on {dev}")
+    if residual is not None:
+        _no_grad(residual)
+        if residual.shape != (M, N) or residual.dtype != dtype or residual.device != dev:
+            raise C.QmoeError("gemm: the residual is [M, N] in the output's dtype, on its device")
+        residual = residual.contiguous()
+    y = torch.empty(M, N, dtype=dtype, device=dev)
+    if M == 0 or N == 0:
+        return y
+    q, xq = prepare(q), prepare(xq)
+    with _on(y):
+        C.call("dq_gemm_nvfp4", C.ptr(q["w"]), C.ptr(q["sca"]), C.ptr(q["s"]), int(q["fmt"] == "nvfp4_rows"),
+               C.ptr(xq["w"]), C.ptr(xq["sca"]), C.ptr(xq["s"]), int(xq["fmt"] == "nvfp4_rows"), M, N, K,
+               2 if residual is not None else _ACTS[act], C.ptr(residual), C.ptr(y), C.DT[dtype], C.stream_of(y))
+    return y
+
+
+def qlinear_a4(q, x, act=None, residual=None):
+    """qlinear with the activations in NVFP4 too: x [..., K] is quantized row by row, then gemm: [..., N] in x.dtype.
+    The result carries the activations' four-bit rounding (about a tenth of a row's norm), for half or less of the
+    time of a bf16 product."""
+    sh = x.shape
+    x2 = x.reshape(-1, sh[-1])
+    if residual is not None:
+        residual = residual.reshape(-1, q["N"])
+    return gemm(q, quantize(x2), x.dtype, act, residual).view(*sh[:-1], q["N"])
+
+
+def gemm_status(device=None, clear=True):
+    """0, or the first error the gemm kernels of the device recorded since the last clear (a wait that ran out: 4, see
+    qmoe_ns.set_wait_cycles); waits for the current stream."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(dev):
+        return int(C.lib().dq_gemm_nvfp4_status(int(clear), torch.cuda.current_stream(dev).cuda_stream))
 
 
 def nbytes(q):

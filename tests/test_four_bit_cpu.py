@@ -1,0 +1,92 @@
+"""What the four-bit operators refuse, checked without a GPU: the C entry points' codes and the Python errors."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import os
+
+    import _qmoe_lib
+    if not os.path.exists(_qmoe_lib.LIB_PATH):
+        import qmoe_build
+        qmoe_build.build()
+    return _qmoe_lib.lib()
+
+
+P = ctypes.c_void_p
+
+
+def test_quantize_arguments(lib):
+    a = P(256)
+
+    def call(x=a, dt=1, ldx=64, M=4, K=64, w=a, sc=a, s=a, atoms=a):
+        return lib.dq_quantize_nvfp4(x, dt, ldx, M, K, 1, w, sc, s, atoms, None)
+
+    assert call(x=None) == 5 and call(w=None) == 5 and call(sc=None) == 5 and call(s=None) == 5
+    assert call(M=0) == 1 and call(K=0) == 1 and call(K=40) == 1 and call(ldx=63) == 1 and call(M=1 << 31) == 1
+    assert call(dt=3) == 6 and call(dt=9) == 6
+    assert call(x=P(257)) == 2 and call(w=P(260)) == 2 and call(atoms=P(258)) == 2 and call(dt=0, x=P(258)) == 2
+    if not torch.cuda.is_available():
+        assert call() == 7 and call(atoms=None) == 7
+
+
+def test_atoms_and_dequant_arguments(lib):
+    a = P(256)
+    assert lib.dq_scale_atoms(None, 4, 64, a, None) == 5
+    assert lib.dq_scale_atoms(a, 0, 64, a, None) == 1 and lib.dq_scale_atoms(a, 4, 65, a, None) == 1
+    assert lib.dq_scale_atoms(a, 4, 64, P(258), None) == 2
+    assert lib.dq_dequant_nvfp4(a, a, a, 1, 4, 64, 3, 2, a, 1, None) == 1
+    assert lib.dq_dequant_nvfp4(a, a, a, 1, 4, 64, 0, 5, a, 1, None) == 1
+    assert lib.dq_dequant_nvfp4(P(257), a, a, 1, 4, 64, 0, 4, a, 1, None) == 2
+    assert lib.dq_dequant_nvfp4(a, a, a, 1, 4, 64, 0, 4, a, 7, None) == 6
+
+
+def test_gemm_arguments(lib):
+    a = P(256)
+
+    def call(w=a, wa=a, x=a, xa=a, M=4, N=8, K=64, ep=0, res=None, y=a, dt=1):
+        return lib.dq_gemm_nvfp4(w, wa, a, 0, x, xa, a, 1, M, N, K, ep, res, y, dt, None)
+
+    assert call(w=None) == 5 and call(xa=None) == 5 and call(y=None) == 5 and call(ep=2) == 5
+    assert call(M=0) == 1 and call(N=0) == 1 and call(K=16) == 1 and call(K=48) == 1 and call(ep=3) == 1
+    assert call(dt=3) == 6
+    assert call(w=P(264)) == 2 and call(xa=P(264)) == 2 and call(y=P(257)) == 2 and call(dt=0, y=P(258)) == 2
+    if not torch.cuda.is_available():
+        assert call() == 7
+
+
+def test_python_refusals():
+    import _qmoe_lib as C
+    import dense_q as D
+    x = torch.zeros(2, 64)
+    for bad in (torch.zeros(64), torch.zeros(2, 40), torch.zeros(2, 0), x, torch.zeros(2, 64, dtype=torch.float64)):
+        with pytest.raises(C.QmoeError):
+            D.quantize(bad)
+    with pytest.raises(C.QmoeError):
+        D.quantize(torch.zeros(0, 64), per_row=False)
+    with pytest.raises(C.QmoeError, match="gradient"):
+        D.quantize(torch.zeros(2, 64, requires_grad=True))
+    rows = {"fmt": "nvfp4_rows", "w": torch.zeros(2, 32, dtype=torch.uint8), "sc": torch.zeros(2, 4, dtype=torch.uint8),
+            "s": torch.ones(2), "N": 2, "K": 64}
+    fp8 = {"fmt": "fp8", "w": torch.zeros(2, 64, dtype=torch.uint8), "s": torch.ones(1), "N": 2, "K": 64}
+    with pytest.raises(C.QmoeError, match="scale per row"):
+        D.gemv(rows, torch.zeros(64))
+    with pytest.raises(C.QmoeError, match="NVFP4"):
+        D.prepare(fp8)
+    with pytest.raises(C.QmoeError, match="NVFP4"):
+        D.gemm(fp8, rows)
+    with pytest.raises(C.QmoeError, match="elements per"):
+        D.gemm({**rows, "K": 128}, rows)
+    with pytest.raises(C.QmoeError, match="32"):
+        D.gemm({**rows, "K": 48}, {**rows, "K": 48})
+    with pytest.raises(C.QmoeError, match="act"):
+        D.gemm(rows, rows, act="gelu")
+    with pytest.raises(C.QmoeError, match="act"):
+        D.gemm(rows, rows, act="relu2", residual=torch.zeros(2, 2, dtype=torch.bfloat16))
+    with pytest.raises(C.QmoeError, match="residual"):
+        D.gemm(rows, rows, residual=torch.zeros(2, 3, dtype=torch.bfloat16))
+    with pytest.raises(C.QmoeError, match="dtype"):
+        D.gemm(rows, rows, dtype=torch.float64)
