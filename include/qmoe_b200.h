@@ -194,6 +194,37 @@ int qmoe_route_decode(const float *logits, const float *bias, int n_experts, int
                       const uint8_t *blocks, int64_t block_stride, const float *s2, int64_t *ids, int32_t *sidx,
                       int64_t *tab, float *s2_sel, float *coef, void *stream);
 
+/* Replaces, for any number of tokens, NemotronHMoE.route_tokens_to_experts (tf:697-720) after the router's linear:
+ * logits [T, n_experts] in x_dtype, rows ld elements apart. score 0: sigmoid(logit), choice = score + bias [n_experts]
+ * (bias may be NULL); 1: the softmax of the row, chosen by the logits (bias NULL). n_group > 1: only the topk_group
+ * groups with the largest sums of their two best choices keep them, the others' are 0 (softmax: -inf). ids [T, top_k]
+ * the largest choices in decreasing order, ties to the lower id, a NaN last; weights [T, top_k] = score, / (their sum +
+ * 1e-20) when norm != 0, * scaling; counts [n_experts]: tokens that chose each expert. n_experts <= 1024, top_k <= 32,
+ * n_group <= 32 groups of at least two. */
+int qmoe_route(const void *logits, int x_dtype, int64_t ld, const float *bias, int64_t T, int n_experts, int top_k,
+               int n_group, int topk_group, int norm, int score, float scaling, int64_t *ids, float *weights,
+               int32_t *counts, void *stream);
+
+/* The gradient of qmoe_route's weights: dlogits [T, n_experts] (contiguous, of x_dtype) from dweights [T, top_k] f32 and
+ * the ids the forward chose (each in [0, n_experts), no two of a row equal). */
+int qmoe_route_backward(const void *logits, int x_dtype, int64_t ld, int64_t T, int n_experts, int top_k, int norm, int score,
+                        float scaling, const int64_t *ids, const float *dweights, void *dlogits, void *stream);
+
+/* No counterpart in the reference (it does not train). The balance loss of T tokens: p = score / sum of the token's
+ * scores, P_e its mean over the T' tokens whose mask byte is not 0 (mask NULL: all), f_e = n_experts * counts_e /
+ * (top_k * T'), *loss = coef * sum_e f_e P_e (0 when T' = 0). ids [T, top_k] int64 (ids_64 != 0) or int32; ids outside
+ * [0, n_experts) and those of masked tokens are not counted. c [n_experts] receives coef * f_e / T' for the backward
+ * pass. The workspace needs no initial value; sums run in a fixed order. */
+size_t qmoe_balance_workspace_bytes(int64_t T, int n_experts);
+int qmoe_balance(const void *logits, int x_dtype, int64_t ld, const void *ids, int ids_64, const uint8_t *mask, int64_t T,
+                 int n_experts, int top_k, int score, float coef, float *loss, int32_t *counts, float *c, void *workspace,
+                 size_t workspace_bytes, void *stream);
+
+/* dlogits [T, n_experts] (contiguous, of x_dtype) = *dloss times the gradient of qmoe_balance's loss, f held fixed; rows
+ * of masked tokens are 0. c from qmoe_balance. */
+int qmoe_balance_backward(const void *logits, int x_dtype, int64_t ld, const uint8_t *mask, int64_t T, int n_experts,
+                          int score, const float *c, const float *dloss, void *dlogits, void *stream);
+
 /* ------------------------------------------------------------------ expert parallelism */
 
 /* No counterpart in the reference (it runs every expert on one GPU). Expert e lives on rank

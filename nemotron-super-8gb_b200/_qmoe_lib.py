@@ -40,6 +40,11 @@ SIGNATURES = {
     "dq_gemv_bf16": (_i, [_p, _p, _i, _i, _i, _i, _i, _p, _p, _p]),
     "dq_gemv_nvfp4_bf16": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _p]),
     "qmoe_route_decode": (_i, [_p, _p, _i, _i, _c.c_float, _i, _p, _i64, _p, _p, _p, _p, _p, _p, _p]),
+    "qmoe_route": (_i, [_p, _i, _i64, _p, _i64, _i, _i, _i, _i, _i, _i, _f, _p, _p, _p, _p]),
+    "qmoe_route_backward": (_i, [_p, _i, _i64, _i64, _i, _i, _i, _i, _f, _p, _p, _p, _p]),
+    "qmoe_balance_workspace_bytes": (_sz, [_i64, _i]),
+    "qmoe_balance": (_i, [_p, _i, _i64, _p, _i, _p, _i64, _i, _i, _i, _f, _p, _p, _p, _p, _sz, _p]),
+    "qmoe_balance_backward": (_i, [_p, _i, _i64, _p, _i64, _i, _i, _p, _p, _p, _p]),
     "qmoe_prefill_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "qmoe_prefill_grouped": (_i, [_p, _i64, _i, _i, _p, _p, _p, _p, _i, _i, _i, _p, _p, _sz, _p]),
     "qmoe_ep_dispatch_pack": (_i, [_p, _i, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p, _p]),

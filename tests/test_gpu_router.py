@@ -1,0 +1,337 @@
+"""The router over many tokens and its balance loss (router.route / balance_loss).
+
+Chosen experts have to equal those of torch's fp32 scores sorted stably (ties to the lower id). Weights, losses and
+gradients are compared with 64-bit formulas: a sigmoid or a softmax term in fp32 is off by a few units of 2^-24 (exp 1
+last place, two roundings more), sums of n positive terms by n 2^-24 at most and far less in a tree; 2^-18 relative to the
+quantities that are subtracted covers them with room for sums of 1024 experts or 4096 tokens."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TOL = 2.0 ** -18
+
+
+def seeded(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def chosen(logits, bias, k, n_group=1, topk_group=1, score="sigmoid"):
+    x = logits.float()
+    c = torch.sigmoid(x) if score == "sigmoid" else x
+    if bias is not None:
+        c = c + bias
+    c = torch.where(torch.isnan(c), -float("inf"), c)
+    if n_group > 1:
+        g = c.view(c.shape[0], n_group, -1)
+        best = torch.sort(g, dim=-1, descending=True)[0][..., :2].sum(-1)
+        keep = torch.zeros_like(best, dtype=torch.bool)
+        keep.scatter_(1, torch.sort(best, dim=-1, descending=True, stable=True)[1][:, :topk_group], True)
+        c = torch.where(keep[..., None], g, 0.0 if score == "sigmoid" else -float("inf")).reshape(c.shape)
+    return torch.sort(c, dim=-1, descending=True, stable=True)[1][:, :k]
+
+
+def weights64(x, ids, scaling, norm, score):
+    s = torch.sigmoid(x) if score == "sigmoid" else torch.softmax(x, -1)
+    w = s.gather(1, ids)
+    return (w / (w.sum(-1, keepdim=True) + 1e-20) if norm else w) * scaling
+
+
+def check_route(logits, bias, k, score="sigmoid", norm=False, groups=(1, 1), scaling=5.0, grad=True):
+    import router as R
+    leaf = logits.detach().clone(memory_format=torch.preserve_format).requires_grad_()
+    ids, w, n = R.route(leaf, bias, top_k=k, scaling=scaling, n_group=groups[0], topk_group=groups[1], norm_topk_prob=norm,
+                        score=score)
+    T, E = logits.shape
+    assert ids.dtype == torch.int64 and n.dtype == torch.int32 and w.dtype == torch.float32
+    assert torch.equal(ids, chosen(logits, bias, k, *groups, score))
+    assert torch.equal(n, torch.bincount(ids.flatten(), minlength=E).to(torch.int32))
+    x = logits.double().requires_grad_()
+    ref = weights64(x, ids, scaling, norm, score)
+    assert torch.allclose(w.double(), ref, rtol=TOL, atol=scaling * 1e-30)
+    if not grad:
+        return
+    dw = torch.randn(T, k, generator=seeded(T + E), device=DEV)
+    got, = torch.autograd.grad(w, leaf, dw)
+    want, = torch.autograd.grad(ref, x, dw.double())
+    assert got.dtype == logits.dtype and got.shape == logits.shape
+    # what the gradient subtracts: |dw| s sums to at most scaling * sum |dw| * max score
+    size = scaling * dw.abs().double().sum(-1, keepdim=True) * ref.abs().amax(-1, keepdim=True) / scaling + 1e-30
+    if norm:
+        size = scaling * dw.abs().double().sum(-1, keepdim=True)
+    half = torch.finfo(logits.dtype).eps / 2
+    tiny = torch.finfo(logits.dtype).smallest_normal * torch.finfo(logits.dtype).eps
+    assert bool(((got.double() - want).abs() <= TOL * size + half * want.abs() + tiny).all())
+
+
+CASES = [(1, 512, 22), (1, 1, 1), (2, 7, 7), (9, 33, 5), (64, 512, 22), (131, 128, 6), (1000, 1024, 32), (5000, 512, 22), (77, 60, 8),
+         (40, 257, 17), (3, 1000, 1)]
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("T,E,k", CASES)
+def test_route(T, E, k, score, norm):
+    g = seeded(T * E + k)
+    x = torch.randn(T, E, generator=g, device=DEV) * 2 - 1
+    bias = torch.randn(E, generator=g, device=DEV) * 0.01 if score == "sigmoid" else None
+    check_route(x, bias, k, score, norm)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_route_of_short_types(dtype, score):
+    """Many equal logits in a row: equal choices go to the lower expert."""
+    x = (torch.randn(300, 200, generator=seeded(3), device=DEV) * 2).to(dtype)
+    check_route(x, None, 12, score)
+    check_route(x, None, 12, score, norm=True)
+
+
+@pytest.mark.parametrize("groups", [(8, 4), (4, 2), (2, 1), (32, 3)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_route_in_groups(groups, score):
+    g = seeded(groups[0])
+    for E in (64, 512, 960):
+        x = torch.randn(50, E, generator=g, device=DEV)
+        bias = torch.randn(E, generator=g, device=DEV) * 0.2 if score == "sigmoid" else None   # some choices below 0
+        check_route(x, bias, min(22, E * groups[1] // groups[0]), score, True, groups)
+
+
+def test_route_ties_and_strange_numbers():
+    E = 96
+    x = torch.zeros(12, E, device=DEV)
+    x[1, 40:] = 1.0
+    x[2] = -200.0                                          # scores of 0
+    x[3] = 200.0                                           # scores of 1
+    x[4, ::2] = -float("inf")
+    x[5, 10], x[5, 90] = float("inf"), -float("inf")
+    x[6, 3:60] = float("nan")
+    x[7] = torch.arange(E, device=DEV) % 3
+    x[8] = -0.0
+    x[8, 50:] = 0.0
+    x[9] = float("nan")
+    x[10] = -torch.arange(E, device=DEV).float()
+    x[11] = 20.0 + torch.arange(E, device=DEV) * 0.1       # scores that differ in the last places, or not at all
+    import router as R
+    for bias in (None, torch.zeros(E, device=DEV), torch.linspace(-1, 1, E, device=DEV)):
+        for k in (1, 22, 32):
+            ids, w, n = R.route(x, bias, top_k=k)
+            assert torch.equal(ids, chosen(x, bias, k))
+            assert torch.equal(n, torch.bincount(ids.flatten(), minlength=E).to(torch.int32))
+            assert torch.equal(w, torch.sigmoid(x).gather(1, ids) * 5.0) or torch.isnan(w).any()
+    ids, _, _ = R.route(x[:9], None, top_k=22, score="softmax")
+    assert torch.equal(ids, chosen(x[:9], None, 22, score="softmax"))
+
+
+def test_route_equals_the_torch_router():
+    """The framework's torch router on the same logits: the same experts, bit-identical weights."""
+    import decode_step as DS
+    import router as R
+    g = seeded(21)
+    x = torch.randn(2000, 256, generator=g, device=DEV)
+    gate = torch.randn(512, 256, generator=g, device=DEV) * 0.05
+    bias = torch.randn(512, generator=g, device=DEV) * 0.01
+    ids, w = DS.route_tokens(x, gate, bias)
+    logits = torch.nn.functional.linear(x, gate)
+    got, gw, _ = R.route(logits, bias)
+    o, p = ids.sort(-1), got.sort(-1)
+    assert torch.equal(o[0], p[0]) and torch.equal(w.gather(1, o[1]), gw.gather(1, p[1]))
+
+
+def test_sigmoid_is_torchs():
+    """The choice is made on fp32 scores: over the whole range they are torch's own bits."""
+    import router as R
+    x = torch.linspace(-30, 30, 1 << 20, device=DEV).view(-1, 32)
+    x = torch.cat([x, torch.randn(1 << 15, 32, generator=seeded(2), device=DEV)])
+    ids, w, _ = R.route(x, None, top_k=32, scaling=1.0)
+    assert torch.equal(w, torch.sigmoid(x).gather(1, ids))
+
+
+def test_route_strides_streams_and_replay():
+    import router as R
+    g = seeded(12)
+    big = torch.randn(128, 600, generator=g, device=DEV)
+    for x in (big[:, 3:515], big[::2, :512], big.t()[:512, :100].t(), big[:1, 5:500], big[:0, :64]):
+        if x.shape[0]:
+            check_route(x, None, 9)
+        else:
+            ids, w, n = R.route(x, None, top_k=9)
+            assert ids.shape == (0, 9) and not n.any()
+    x = big[:, :512].contiguous()
+    want = R.route(x, None)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = R.route(x, None)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    buf = x.clone()
+    with torch.cuda.graph(graph):
+        out = R.route(buf, None)
+    for y in (x, big[:, 50:562].contiguous(), x):
+        buf.copy_(y)
+        graph.replay()
+        graph.replay()                                     # counts start from zero in every replay
+        assert all(torch.equal(a, b) for a, b in zip(out, R.route(y, None)))
+
+
+# ------------------------------------------------------------------------------------------------ balance loss
+def loss64(x, ids, mask, score, coef):
+    T, E = x.shape
+    keep = torch.ones(T, dtype=torch.bool, device=DEV) if mask is None else mask
+    rows = int(keep.sum())
+    i = ids[keep].long().flatten()
+    i = i[(i >= 0) & (i < E)]
+    n = torch.bincount(i, minlength=E)
+    if rows == 0:
+        return x.sum() * 0, n, torch.zeros(E, dtype=torch.float64, device=DEV)
+    f = n.double() * E / (ids.shape[1] * rows)
+    s = torch.sigmoid(x) if score == "sigmoid" else torch.softmax(x, -1)
+    p = (s / s.sum(-1, keepdim=True))[keep]
+    return coef * (f * p.mean(0)).sum(), n, coef * f / rows
+
+
+def check_balance(logits, ids, mask=None, score="sigmoid", coef=1.0):
+    import router as R
+    leaf = logits.detach().clone().requires_grad_()
+    loss, n = R.balance_loss(leaf, ids, mask, score, coef)
+    x = logits.double()
+    if mask is not None:
+        x = torch.where(mask[:, None], x, 0.0)             # what masked rows hold does not matter
+    x.requires_grad_()
+    want, n64, c = loss64(x, ids, mask, score, coef)
+    assert torch.equal(n, n64.to(torch.int32)) and loss.shape == () and loss.dtype == torch.float32
+    assert abs(float(loss) - float(want)) <= TOL * abs(float(want))
+    got, = torch.autograd.grad(loss * 3.0, leaf)
+    ref, = torch.autograd.grad(want * 3.0, x)
+    s = torch.sigmoid(x) if score == "sigmoid" else torch.softmax(x, -1)
+    p = s / s.sum(-1, keepdim=True)
+    half = torch.finfo(logits.dtype).eps / 2
+    tiny = torch.finfo(logits.dtype).smallest_normal * torch.finfo(logits.dtype).eps
+    size = 3 * p * (c + (c * p).sum(-1, keepdim=True))     # the two terms that are subtracted
+    assert got.dtype == logits.dtype
+    assert bool(((got.double() - ref).abs() <= TOL * size + half * ref.abs() + tiny).all())
+    if mask is not None:
+        assert not got[~mask].any()
+    return loss.detach(), got
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 512, 22), (5, 7, 2), (64, 33, 32), (300, 128, 6), (1001, 512, 22), (4096, 1024, 8), (9, 257, 40)])
+def test_balance(T, E, k, score, dtype):
+    g = seeded(T + E)
+    x = (torch.randn(T, E, generator=g, device=DEV) * 1.5).to(dtype)
+    ids = torch.topk(x.float(), min(k, E), -1)[1]
+    check_balance(x, ids, None, score, 0.01)
+    mask = torch.rand(T, generator=g, device=DEV) < 0.6
+    check_balance(x, ids.to(torch.int32), mask, score)
+
+
+def test_balance_masks_and_odd_ids():
+    g = seeded(31)
+    x = torch.randn(50, 64, generator=g, device=DEV)
+    ids = torch.randint(0, 64, (50, 5), generator=g, device=DEV)
+    ids[3] = -1
+    ids[4, 2] = 64
+    ids[5] = 7                                             # the same expert five times
+    mask = torch.zeros(50, dtype=torch.bool, device=DEV)
+    loss, grad = check_balance(x, ids, mask)               # nothing left
+    assert float(loss) == 0.0 and not grad.any()
+    mask[17] = True
+    check_balance(x, ids, mask)                            # one token
+    mask[:40] = True
+    y = x.clone()
+    y[40:] = float("nan")
+    y[45] = float("inf")
+    y[46] = torch.finfo(torch.float32).min
+    a, b = check_balance(y, ids, mask), check_balance(x, ids, mask)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    import router as R
+    loss, n = R.balance_loss(x[:0], ids[:0])
+    assert float(loss) == 0.0 and not n.any()
+
+
+def test_even_load_gives_one():
+    import router as R
+    ids = torch.arange(512, device=DEV).view(64, 8)
+    loss, n = R.balance_loss(torch.zeros(64, 512, device=DEV), ids)
+    assert abs(float(loss) - 1.0) <= TOL and bool((n == 1).all())
+
+
+def test_gradients_against_differences():
+    """Central differences of the forward passes' own values, in directions of random signs. With step h the fp32 values'
+    error 2^-22 |L| / h and the third derivative's h^2 stay below 1 % of the directional derivative's scale."""
+    import router as R
+    g = seeded(41)
+    x = torch.randn(16, 24, generator=g, device=DEV)
+    dw = torch.randn(16, 4, generator=g, device=DEV)
+    h = 2.0 ** -7
+    for score in ("sigmoid", "softmax"):
+        ids0, _, _ = R.route(x, None, top_k=4, score=score)
+
+        def weights(y):
+            return weights64(y.double(), ids0, 5.0, True, score)
+
+        leaf = x.clone().requires_grad_()
+        ids, w, _ = R.route(leaf, None, top_k=4, norm_topk_prob=True, score=score)
+        grad = torch.autograd.grad(w, leaf, dw)[0]
+        lossg = torch.autograd.grad(R.balance_loss(leaf, ids0, score=score)[0], leaf)[0]
+        for seed in range(4):
+            d = torch.sign(torch.randn(16, 24, generator=seeded(seed), device=DEV))
+            num = ((weights(x + h * d) - weights(x - h * d)) * dw).sum() / (2 * h)
+            assert abs(float(num) - float((grad.double() * d).sum())) <= 0.01 * float((grad.abs()).sum())
+            up, down = (float(R.balance_loss(x + v * d, ids0, score=score)[0]) for v in (h, -h))
+            assert abs((up - down) / (2 * h) - float((lossg.double() * d).sum())) <= 0.01 * float(lossg.abs().sum())
+
+
+def test_training_step_of_both_and_reruns():
+    """One step's gradient through the weights and the loss together, twice: the same bits; and as a captured graph."""
+    import router as R
+    g = seeded(51)
+    x = torch.randn(700, 512, generator=g, device=DEV)
+    dw = torch.randn(700, 22, generator=g, device=DEV)
+
+    def step(v):
+        leaf = v.detach().requires_grad_()
+        ids, w, n = R.route(leaf, None, norm_topk_prob=True)
+        loss, m = R.balance_loss(leaf, ids, coef=0.01)
+        return torch.autograd.grad([w, loss], leaf, [dw, torch.ones_like(loss)])[0], n, m, loss.detach()
+
+    a, b = step(x), step(x)
+    assert all(torch.equal(u, v) for u, v in zip(a, b)) and torch.equal(a[1], a[2])
+    y = x.double().requires_grad_()
+    ids = chosen(x, None, 22)
+    ref = torch.autograd.grad([weights64(y, ids, 5.0, True, "sigmoid"), loss64(y, ids, None, "sigmoid", 0.01)[0]], y,
+                              [dw.double(), torch.ones((), dtype=torch.float64, device=DEV)])[0]
+    assert bool(((a[0].double() - ref).abs() <= 2 * TOL * 5 * dw.abs().double().sum(-1, keepdim=True)).all())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    buf = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(buf)
+    for v in (x, x.flip(0)):
+        buf.copy_(v)
+        graph.replay()
+        assert all(torch.equal(p, q) for p, q in zip(out, step(v)))
+
+
+def test_only_what_is_asked_for_is_differentiated():
+    import router as R
+    x = torch.randn(8, 16, generator=seeded(1), device=DEV, requires_grad=True)
+    ids, w, n = R.route(x, None, top_k=2)
+    assert not ids.requires_grad and not n.requires_grad and w.requires_grad
+    w.sum().backward()                                     # an expanded gradient
+    assert x.grad is not None
+    with torch.no_grad():
+        assert not R.route(x, None, top_k=2)[1].requires_grad
+    bias = torch.zeros(16, device=DEV, requires_grad=True)
+    R.route(x, bias, top_k=2)[1].sum().backward()
+    assert bias.grad is None
