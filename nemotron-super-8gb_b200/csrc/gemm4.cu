@@ -25,27 +25,21 @@ constexpr int MAX_SPLIT = 8;
 
 __device__ int g_status;             // first error of this device's calls since it was last cleared
 
-template <int TN> struct Plan {
-    static constexpr int NA = (TN + 127) / 128;        // scale atoms of the tokens per k-step
+template <int TN> struct Plan {   // TN <= 128: a stage holds one atom of token scales per k-step
     static constexpr int B_BYTES = TN * ROWB;
-    static constexpr int SFB_BYTES = NA * 4 * ATOM;
     static constexpr int OFF_B = A_BYTES, OFF_SFA = OFF_B + B_BYTES, OFF_SFB = OFF_SFA + SFA_BYTES;
-    static constexpr int STAGE = (OFF_SFB + SFB_BYTES + 1023) / 1024 * 1024;
+    static constexpr int STAGE = (OFF_SFB + SFA_BYTES + 1023) / 1024 * 1024;
     static constexpr int STAGES = 221184 / STAGE < 8 ? 221184 / STAGE : 8;
     static constexpr int OFF_BAR = STAGES * STAGE;
     static constexpr int NBAR = 2 * STAGES + 5;
     static constexpr int OFF_MISC = OFF_BAR + (NBAR * 8 + 15) / 16 * 16;
     static constexpr int SMEM = OFF_MISC + 16 + 1024;
     static_assert(SMEM <= 232448, "fits the 227 KB opt-in");
-    // Tensor memory: two accumulators of TN columns and two scale slots. At TN = 256 the accumulators overlap in 96
-    // columns (0..255 and 160..415), which the epilogue drains first, so that the next tile starts before it is done.
-    static constexpr int ACC1 = TN == 256 ? 160 : TN;
-    static constexpr int SF_COL = ACC1 + TN;
-    static constexpr int SF_SLOT = 4 * 4 * (1 + NA);
+    // Tensor memory: two accumulators of TN columns and two scale slots.
+    static constexpr int SF_COL = 2 * TN;
+    static constexpr int SF_SLOT = 4 * 4 * 2;
     static constexpr int NEED = SF_COL + 2 * SF_SLOT;
     static constexpr int COLS = NEED <= 128 ? 128 : NEED <= 256 ? 256 : 512;
-    static_assert(NEED <= 512, "tensor memory");
-    static constexpr int LAG = TN == 256 ? 1 : 2;      // tile t's MMAs wait for the release of tile t - LAG
 };
 
 struct Params {
@@ -59,6 +53,25 @@ struct Params {
     void *y;
     long long wait;
 };
+
+// The load and MMA warps run their loops with all lanes, so that addresses and descriptors stay in uniform registers;
+// only the instruction itself is one lane's. (From a loop that one lane runs alone, every such instruction cost 100 to
+// 150 cycles to issue: 8192 x 12288 x 4096 took 413 us.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(v));
+    return v != 0;
+}
+
+// Bounded wait of a whole warp; the result is the same in every lane.
+__device__ __forceinline__ bool all_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, long long limit) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0) ok = lane_wait(bar, parity, abort_flag, &g_status, limit);
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    if (ok) mbar_try_wait(bar, parity);   // a completed phase: the acquire of the other lanes
+    return ok;
+}
 
 __device__ __forceinline__ void cp_sf(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
@@ -83,11 +96,10 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
     return v;
 }
 
-// The product is rounded before a residual is added to it: no fused multiply-add.
-__device__ __forceinline__ float scaled(float v, float sx, float sw) { return __fmul_rn(__fmul_rn(v, sx), sw); }
-
-// One result: the linear's value rounded to the output type, then (in fp32, rounded again) its squared ReLU or the
-// sum with the residual, as the unfused operators round.
+// Results. The linear's value is rounded to the output type, then (in fp32, rounded again) its squared ReLU or the sum
+// with the residual, as the unfused operators round (no fused multiply-add). EPI is a template argument and its switch
+// stands outside the unrolled columns: with it inside, the epilogue's code no longer fitted the instruction cache and
+// 32 columns took 2,400 cycles instead of 200.
 template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
@@ -96,16 +108,29 @@ __device__ __forceinline__ float wide(float v) { return v; }
 __device__ __forceinline__ float wide(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float wide(__half v) { return __half2float(v); }
 
-template <typename T> __device__ __forceinline__ void store(const Params &p, int64_t at, float v) {
-    T o = narrow<T>(v);
-    if (p.epilogue == 1) {
-        float b = wide(o);
-        b = b > 0.f ? b : (b != b ? b : 0.f);
-        o = narrow<T>(b * b);
-    } else if (p.epilogue == 2) {
-        o = narrow<T>(wide(o) + wide(static_cast<const T *>(p.res)[at]));
+// sx * sw * v and its epilogue, before the last rounding.
+template <typename T, int EPI> __device__ __forceinline__ float finish(float v, float sx, float sw, float res) {
+    v = __fmul_rn(__fmul_rn(v, sx), sw);
+    if (EPI == 1) {
+        const float o = wide(narrow<T>(v)), r = o > 0.f ? o : (o != o ? o : 0.f);
+        return __fmul_rn(r, r);
     }
-    static_cast<T *>(p.y)[at] = o;
+    return EPI == 2 ? __fadd_rn(wide(narrow<T>(v)), res) : v;
+}
+
+template <typename T, int EPI> __device__ __forceinline__ void store_one(void *y, const void *res, int64_t at, float v, float sx, float sw) {
+    static_cast<T *>(y)[at] = narrow<T>(finish<T, EPI>(v, sx, sw, EPI == 2 ? wide(static_cast<const T *>(res)[at]) : 0.f));
+}
+
+// 32 tokens' columns of one weight row (a lane): element j at y[at + j * N], for the first `left` of them. Lane j of the
+// warp holds token j's scale in sx.
+template <typename T, int EPI>
+__device__ __forceinline__ void store_columns(void *y, const void *res, int64_t at, int64_t N, bool in, int left, const float (&v)[32], float sx, float sw) {
+#pragma unroll
+    for (int j = 0; j < 32; j++) {
+        const float s = __shfl_sync(0xffffffffu, sx, j);
+        if (in && j < left) store_one<T, EPI>(y, res, at + j * N, v[j], s, sw);
+    }
 }
 
 template <int TN, typename T>
@@ -120,7 +145,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t *full = reinterpret_cast<uint64_t *>(sm + P::OFF_BAR);
     uint64_t *empty = full + S;
     uint64_t *acc_full = empty + S;      // [2]
-    uint64_t *acc_free = acc_full + 2;   // [2] tile t (at t & 1): the columns that tile t + LAG needs are drained
+    uint64_t *acc_free = acc_full + 2;   // [2] the accumulator is drained
     uint64_t *drain = acc_free + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + P::OFF_MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(sm + P::OFF_MISC + 8);
@@ -158,33 +183,34 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     if (warp == 4) {
         // ------------------------------------------------------------ loads
-        if (lane == 0) {
+        {
             bool ok = true;
             for (int i = first; i < p.ntiles && ok; i += step) {
                 const int n0 = i % p.nbn * BM, m0 = i / p.nbn * TN;
                 const uint8_t *fa = p.sfa + (int64_t)(n0 >> 7) * p.nks * ATOM, *fb = p.sfb + (int64_t)(m0 >> 7) * p.nks * ATOM;
-                const int na = P::NA > 1 && m0 + 128 >= p.M ? 1 : P::NA;   // no tokens, and no atoms, past M
                 for (int kt = k0; kt < k1; kt++, q++) {
                     const int s = q % S;
-                    if (!lane_wait(&empty[s], ((q / S) & 1) ^ 1, abort_flag, &g_status, p.wait)) {
+                    if (!all_wait(&empty[s], ((q / S) & 1) ^ 1, abort_flag, p.wait)) {
                         ok = false;
                         break;
                     }
                     uint8_t *st = sm + s * P::STAGE;
                     const uint32_t sf = (uint32_t)min(4, p.nks - 4 * kt) * ATOM;
-                    mbar_expect_tx(&full[s], A_BYTES + P::B_BYTES + sf * (1 + na));
-                    tma_load_2d(st, &tm_a, kt * ROWB, n0, &full[s]);
-                    tma_load_2d(st + P::OFF_B, &tm_b, kt * ROWB, m0, &full[s]);
-                    bulk_g2s_nohint(st + P::OFF_SFA, fa + (int64_t)kt * SFA_BYTES, sf, &full[s]);
-                    for (int a = 0; a < na; a++)
-                        bulk_g2s_nohint(st + P::OFF_SFB + a * SFA_BYTES, fb + ((int64_t)a * p.nks + 4 * kt) * ATOM, sf, &full[s]);
+                    if (elect_one()) {
+                        mbar_expect_tx(&full[s], A_BYTES + P::B_BYTES + 2 * sf);
+                        tma_load_2d(st, &tm_a, kt * ROWB, n0, &full[s]);
+                        tma_load_2d(st + P::OFF_B, &tm_b, kt * ROWB, m0, &full[s]);
+                        bulk_g2s_nohint(st + P::OFF_SFA, fa + (int64_t)kt * SFA_BYTES, sf, &full[s]);
+                        bulk_g2s_nohint(st + P::OFF_SFB, fb + (int64_t)kt * SFA_BYTES, sf, &full[s]);
+                    }
+                    __syncwarp();
                 }
             }
         }
         __syncwarp();
     } else if (warp == 5) {
         // ------------------------------------------------------------ scales to tensor memory, MMAs
-        if (lane == 0) {
+        {
             const uint64_t dbase = smem_desc(0, 16, 1024, 2);   // K-major, 128-byte swizzle
             const uint64_t fbase = smem_desc(0, 16, 128, 0);    // an atom: 32 rows of 16 bytes
             int t = 0;
@@ -192,13 +218,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int i = first; i < p.ntiles && ok; i += step, t++) {
                 const int m0 = i / p.nbn * TN;
                 const uint32_t idesc = instr_desc_nvfp4((min(TN, p.M - m0) + 15) & ~15);
-                const int f = t - P::LAG;
-                if (f >= 0 && !lane_wait(&acc_free[f & 1], (f >> 1) & 1, abort_flag, &g_status, p.wait)) break;
+                const int f = t - 2;   // the tile that had this accumulator before
+                if (f >= 0 && !all_wait(&acc_free[f & 1], (f >> 1) & 1, abort_flag, p.wait)) break;
                 tc_fence_after();
-                const uint32_t d = tmem + (t & 1) * P::ACC1;
+                const uint32_t d = tmem + (t & 1) * TN;
                 for (int kt = k0; kt < k1; kt++, q++) {
                     const int s = q % S;
-                    if (!lane_wait(&full[s], (q / S) & 1, abort_flag, &g_status, p.wait)) {
+                    if (!all_wait(&full[s], (q / S) & 1, abort_flag, p.wait)) {
                         ok = false;
                         break;
                     }
@@ -206,20 +232,24 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const uint32_t st = sbase + s * P::STAGE;
                     const uint32_t slot = tmem + P::SF_COL + (q & 1) * P::SF_SLOT;
                     const int nk = min(4, p.nks - 4 * kt);
-                    for (int kk = 0; kk < nk; kk++) {
-                        const uint32_t c = slot + kk * 4 * (1 + P::NA);
-                        cp_sf(c, fbase + ((st + P::OFF_SFA + kk * ATOM) >> 4));
+                    if (elect_one()) {
 #pragma unroll
-                        for (int a = 0; a < P::NA; a++)
-                            cp_sf(c + 4 + 4 * a, fbase + ((st + P::OFF_SFB + a * SFA_BYTES + kk * ATOM) >> 4));
+                        for (int kk = 0; kk < 4; kk++) {
+                            if (kk >= nk) break;
+                            cp_sf(slot + 8 * kk, fbase + ((st + P::OFF_SFA + kk * ATOM) >> 4));
+                            cp_sf(slot + 8 * kk + 4, fbase + ((st + P::OFF_SFB + kk * ATOM) >> 4));
+                        }
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++) {
+                            if (kk >= nk) break;
+                            const uint32_t c = slot + 8 * kk;
+                            mma_nvfp4(d, dbase + (st >> 4) + 2 * kk, dbase + ((st + P::OFF_B) >> 4) + 2 * kk, idesc, (kt > k0) | (kk > 0), c, c + 4);
+                        }
+                        mma_commit(&empty[s]);
+                        if (kt == k1 - 1) mma_commit(&acc_full[t & 1]);
                     }
-                    for (int kk = 0; kk < nk; kk++) {
-                        const uint32_t c = slot + kk * 4 * (1 + P::NA);
-                        mma_nvfp4(d, dbase + (st >> 4) + 2 * kk, dbase + ((st + P::OFF_B) >> 4) + 2 * kk, idesc, (kt > k0) | (kk > 0), c, c + 4);
-                    }
-                    mma_commit(&empty[s]);
+                    __syncwarp();
                 }
-                mma_commit(&acc_full[t & 1]);
             }
         }
         __syncwarp();
@@ -230,7 +260,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!warp_wait_bo(&acc_full[t & 1], (t >> 1) & 1, lane, abort_flag, &g_status, p.wait)) break;
             tc_fence_after();
             const int n = i % p.nbn * BM + tid, m0 = i / p.nbn * TN, cols = min(TN, p.M - m0);
-            const uint32_t d = tmem + (t & 1) * P::ACC1 + ((uint32_t)(warp * 32) << 16);
+            const uint32_t d = tmem + (t & 1) * TN + ((uint32_t)(warp * 32) << 16);
             if (split > 1) {
                 float *dump = reinterpret_cast<float *>(sm);   // every stage has been read
                 for (int c0 = 0; c0 < cols; c0 += 32) {
@@ -243,21 +273,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                 break;
             }
             const float sw = n < p.N ? p.sw[(int64_t)n * p.sw_step] : 0.f;
-            // TN = 256: the 96 shared columns first (accumulator 0: its last, accumulator 1: its first)
-            for (int u = 0; u < TN; u += 32) {
-                const int c0 = TN == 256 && !(t & 1) ? (u < 96 ? 160 + u : u - 96) : u;
+#pragma unroll 1
+            for (int c0 = 0; c0 < TN; c0 += 32) {
                 float v[32];
-                if (c0 < cols) tmem_ld32(d + c0, v);
-                if (u == (TN == 256 ? 64 : (TN - 1) / 32 * 32)) {
+                const int left = cols - c0;
+                if (left > 0) tmem_ld32(d + c0, v);
+                if (c0 + 32 >= TN) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&acc_free[t & 1]);
                 }
-                if (n < p.N)
-#pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (c0 + j < cols)
-                            store<T>(p, (int64_t)(m0 + c0 + j) * p.N + n, scaled(v[j], p.sx[(int64_t)(m0 + c0 + j) * p.sx_step], sw));
+                if (left <= 0) continue;
+                const float sx = p.sx[(int64_t)(m0 + c0 + min(lane, left - 1)) * p.sx_step];
+                const int64_t at = (int64_t)(m0 + c0) * p.N + n;
+                if (p.epilogue == 0) store_columns<T, 0>(p.y, p.res, at, p.N, n < p.N, left, v, sx, sw);
+                else if (p.epilogue == 1) store_columns<T, 1>(p.y, p.res, at, p.N, n < p.N, left, v, sx, sw);
+                else store_columns<T, 2>(p.y, p.res, at, p.N, n < p.N, left, v, sx, sw);
             }
         }
     }
@@ -271,7 +302,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             float v = 0.f;
             for (int r = 0; r < split; r++) v += ld_cluster(sbase + e * 4, r);
             const int n = n0 + e % BM, m = m0 + e / BM;
-            if (n < p.N) store<T>(p, (int64_t)m * p.N + n, scaled(v, p.sx[(int64_t)m * p.sx_step], p.sw[(int64_t)n * p.sw_step]));
+            if (n < p.N) {
+                const float sx = p.sx[(int64_t)m * p.sx_step], sw = p.sw[(int64_t)n * p.sw_step];
+                const int64_t at = (int64_t)m * p.N + n;
+                if (p.epilogue == 0) store_one<T, 0>(p.y, p.res, at, v, sx, sw);
+                else if (p.epilogue == 1) store_one<T, 1>(p.y, p.res, at, v, sx, sw);
+                else store_one<T, 2>(p.y, p.res, at, v, sx, sw);
+            }
         }
         cluster_sync();   // no CTA leaves while another reads its sums
     }
@@ -282,7 +319,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         // its last use, since an earlier one was consumed before the stage was loaded again. MMAs: one more commit.
         if (warp == 4)
             for (uint32_t u = q > (uint32_t)S ? q - S : 0; u < q; u++) mbar_wait(&full[u % S], (u / S) & 1);
-        if (warp == 5) {
+    }
+    if (warp == 5 && *abort_flag) {   // the lane that issued the MMAs: elect picks the same one every time
+        if (elect_one()) {
             mma_commit(drain);
             mbar_wait(drain, 0);
         }
@@ -291,6 +330,361 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 5) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::COLS) : "memory");
+    }
+}
+
+// ------------------------------------------------------------------------------------------ pairs of CTAs
+// The same product for many tokens: a cluster of two CTAs computes 256 x TN with cta_group::2 MMAs. Each CTA holds 128
+// rows of the one operand and half of the other's TN, so that a stage costs each SM 70 KB of shared-memory traffic
+// for 512 cycles of tensor work at TN = 256; one CTA alone on 128 x 256 needs 102 KB, which is what bounded it.
+// Which operand has the 256 rows (the lanes of tensor memory) is the caller's choice: with the tokens there, a thread
+// holds consecutive columns of one row of y and stores 32 bytes at a time; with the weights there, a warp's lanes are
+// consecutive in a row of y, which suits rows of y that are not 32-byte aligned.
+// What is left is issue: a stage is 4 MMAs of 128 cycles and 12 scale copies, and one warp needs about 30 cycles for a
+// copy and 40 for an MMA. So one warp issues the copies, up to two stages ahead, and another the MMAs.
+constexpr int PAIR_THREADS = 224;   // warps 0..3 epilogue, 4 loads, 5 MMA, 6 scale copies
+
+template <int TN> struct PairPlan {
+    static constexpr int NA = (TN + 127) / 128;
+    static constexpr int B_BYTES = TN / 2 * ROWB;
+    static constexpr int OFF_B = A_BYTES, OFF_SFA = OFF_B + B_BYTES, OFF_SFB = OFF_SFA + SFA_BYTES;
+    static constexpr int BYTES = OFF_SFB + NA * SFA_BYTES;
+    static constexpr int STAGE = (BYTES + 1023) / 1024 * 1024;
+    static constexpr int STAGES = 221184 / STAGE < 8 ? 221184 / STAGE : 8;
+    static constexpr int OFF_BAR = STAGES * STAGE;
+    static constexpr int NBAR = 2 * STAGES + 7;
+    static constexpr int OFF_MISC = OFF_BAR + (NBAR * 8 + 15) / 16 * 16;
+    static constexpr int SMEM = OFF_MISC + 16 + 1024;
+    static_assert(SMEM <= 232448, "fits the 227 KB opt-in");
+    static constexpr int ACC1 = TN == 256 ? 160 : TN;   // as Plan: at TN = 256 the accumulators share 96 columns
+    static constexpr int SF_COL = ACC1 + TN;
+    static constexpr int SF_SLOT = 4 * 4 * (1 + NA);
+    static constexpr int LAG = TN == 256 ? 1 : 2;
+    static_assert(SF_COL + 2 * SF_SLOT <= 512, "tensor memory");
+};
+
+struct PairParams {
+    const float *sa, *sb;   // scales of the lanes' and of the columns' operand
+    int sa_step, sb_step;
+    int A, B;               // rows of the two operands
+    int nks, nst, nba, ntiles;
+    int tokens_on_lanes;
+    int N;                  // row length of y
+    const void *res;
+    void *y;
+    long long wait;
+};
+
+__device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+// Descriptors in halves: the upper is constant, the lower (address / 16 and the leading offset) takes one addition.
+constexpr uint32_t LO = 1u << 16, HI_SF = (128u >> 4) | (1u << 14), HI_TILE = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void cp_sf_pair(uint32_t taddr, uint32_t lo) {
+    asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\ttcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n\t}" ::"r"(taddr), "r"(lo), "r"(HI_SF)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t sfa, uint32_t sfb) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 a, {%1, %7};\n\tmov.b64 b, {%2, %7};\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.block16 [%0], a, b, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb), "r"(HI_TILE)
+        : "memory");
+}
+// Arrives on both CTAs' barrier at this offset once the MMAs issued so far have completed.
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+__device__ __forceinline__ void commit_one(uint64_t *bar) {   // on the issuing CTA's barrier alone
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t in_leader(const void *p) {   // the same place in the pair's first CTA
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
+
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<float>(float, float) { return 0; }
+__device__ __forceinline__ float2 unpack2(uint32_t v, __nv_bfloat16) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
+__device__ __forceinline__ float2 unpack2(uint32_t v, __half) { return __half22float2(as_h2(v)); }
+__device__ __forceinline__ float2 unpack2(uint32_t, float) { return make_float2(0.f, 0.f); }
+
+__device__ __forceinline__ void st32(void *p, const uint32_t (&v)[8]) {   // 32 bytes, 32-byte aligned
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void ld32(const void *p, uint32_t (&v)[8]) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "l"(p));
+}
+
+// 32 weight rows' columns of one token (a lane): y[at ..], for the first `left` of them, 32 bytes at a time (left, like the
+// row length, is a multiple of those). sw: one for all, or lane j's register holds column j's.
+template <typename T, int EPI>
+__device__ __forceinline__ void store_run(void *y, const void *res, int64_t at, bool in, int left, const float (&v)[32], float sx, float sw, bool each) {
+    constexpr int EPV = 32 / sizeof(T);   // elements per store
+#pragma unroll
+    for (int u = 0; u < 32 / EPV; u++) {
+        const bool live = in && u * EPV < left;
+        uint32_t r[8] = {}, o[8];
+        if (EPI == 2 && live) ld32(static_cast<const T *>(res) + at + u * EPV, r);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if constexpr (sizeof(T) == 4) {
+                const int c = u * EPV + j;
+                o[j] = __float_as_uint(finish<T, EPI>(v[c], sx, each ? __shfl_sync(0xffffffffu, sw, c) : sw, __uint_as_float(r[j])));
+            } else {
+                const int c = u * EPV + 2 * j;
+                const float2 q = unpack2(r[j], T{});
+                const float lo = finish<T, EPI>(v[c], sx, each ? __shfl_sync(0xffffffffu, sw, c) : sw, q.x);
+                const float hi = finish<T, EPI>(v[c + 1], sx, each ? __shfl_sync(0xffffffffu, sw, c + 1) : sw, q.y);
+                o[j] = pack2<T>(lo, hi);
+            }
+        }
+        if (live) st32(static_cast<T *>(y) + at + u * EPV, o);
+    }
+}
+
+template <int TN, typename T, int EPI>
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+    pair_kernel(const PairParams p, const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                const __grid_constant__ CUtensorMap tm_sa, const __grid_constant__ CUtensorMap tm_sb) {
+    using P = PairPlan<TN>;
+    constexpr int S = P::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    uint8_t *sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+    const uint32_t sbase = smem_u32(sm);
+    uint64_t *full = reinterpret_cast<uint64_t *>(sm + P::OFF_BAR);   // the first CTA's count both CTAs' copies
+    uint64_t *empty = full + S;
+    uint64_t *acc_full = empty + S;      // [2]
+    uint64_t *acc_free = acc_full + 2;   // [2], the first CTA's
+    uint64_t *sf_full = acc_free + 2;    // [2], the first CTA's: a slot's scales are in tensor memory
+    uint64_t *drain = sf_full + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + P::OFF_MISC);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(sm + P::OFF_MISC + 8);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = blockIdx.x & 1, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+    if (tid == 0) {
+        for (int s = 0; s < S; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&acc_full[0], 1);
+        mbar_init(&acc_full[1], 1);
+        mbar_init(&acc_free[0], 8);
+        mbar_init(&acc_free[1], 8);
+        mbar_init(&sf_full[0], 1);
+        mbar_init(&sf_full[1], 1);
+        mbar_init(drain, 2);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();   // both CTAs' barriers exist before either is signalled
+    tc_fence_after();
+    constexpr uint32_t tmem = 0;   // all 512 columns are this CTA's: they start at column 0
+    uint32_t q = 0;                // stages loaded
+
+    if (warp == 4) {
+        // ------------------------------------------------------------ loads: each CTA its own half of the stage
+        {
+            bool ok = true;
+            for (int i = first; i < p.ntiles && ok; i += step) {
+                const int a0 = i % p.nba * 256 + rank * 128, b0 = i / p.nba * TN;
+                const int fa = (a0 >> 7) * p.nks, fb = (b0 >> 7) * p.nks;
+                for (int kt = 0; kt < p.nst; kt++, q++) {
+                    const int s = q % S;
+                    if (!all_wait(&empty[s], ((q / S) & 1) ^ 1, abort_flag, p.wait)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *st = sm + s * P::STAGE;
+                    const uint32_t bar = in_leader(&full[s]);
+                    if (elect_one()) {
+                        if (rank == 0) mbar_expect_tx(&full[s], 2 * P::BYTES);
+                        tma_load_2d_pair(st, &tm_a, kt * ROWB, a0, bar);
+                        tma_load_2d_pair(st + P::OFF_B, &tm_b, kt * ROWB, b0 + rank * (TN / 2), bar);
+                        tma_load_2d_pair(st + P::OFF_SFA, &tm_sa, 0, fa + 4 * kt, bar);
+#pragma unroll
+                        for (int a = 0; a < P::NA; a++)
+                            tma_load_2d_pair(st + P::OFF_SFB + a * SFA_BYTES, &tm_sb, 0, fb + a * p.nks + 4 * kt, bar);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 5) {
+        // ------------------------------------------------------------ MMAs: the first CTA's warp drives both tensor cores
+        if (rank == 0) {
+            const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | (16u << 24);   // M = 256
+            uint32_t u = 0;
+            int s = 0, t = 0;
+            bool ok = true;
+            for (int i = first; i < p.ntiles && ok; i += step, t++) {
+                const uint32_t d = tmem + (t & 1) * P::ACC1;
+                const int f = t - P::LAG;
+                if (f >= 0 && !all_wait(&acc_free[f & 1], (f >> 1) & 1, abort_flag, p.wait)) break;
+                tc_fence_after();
+                for (int kt = 0; kt < p.nst; kt++, u++) {
+                    if (!all_wait(&sf_full[u & 1], (u >> 1) & 1, abort_flag, p.wait)) {   // and so are the stage's codes
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = ((sbase + s * P::STAGE) >> 4) + LO, c = tmem + P::SF_COL + (u & 1) * P::SF_SLOT;
+                    const int nk = min(4, p.nks - 4 * kt);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++) {
+                            if (kk >= nk) break;
+                            mma_pair(d, a + 2 * kk, a + (P::OFF_B >> 4) + 2 * kk, idesc, (kt > 0) | (kk > 0), c + kk * 4 * (1 + P::NA), c + kk * 4 * (1 + P::NA) + 4);
+                        }
+                        commit_pair(&empty[s]);
+                        if (kt == p.nst - 1) commit_pair(&acc_full[t & 1]);
+                    }
+                    __syncwarp();
+                    s = s + 1 == S ? 0 : s + 1;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 6) {
+        // ------------------------------------------------------------ scales to tensor memory, for both CTAs
+        if (rank == 0) {
+            const uint32_t total = (uint32_t)((p.ntiles - first + step - 1) / step) * p.nst;
+            uint32_t ph = 0, last = 0;   // parity of stage s's current use, and of the use two stages before
+            int s = 0, s2 = 0, kt = 0;
+            for (uint32_t u = 0; u < total; u++) {
+                if (!all_wait(&full[s], ph, abort_flag, p.wait)) break;
+                if (u >= 2) {   // the slot's last MMAs have completed
+                    if (!all_wait(&empty[s2], last, abort_flag, p.wait)) break;
+                    if (++s2 == S) s2 = 0, last ^= 1;
+                }
+                tc_fence_after();
+                const uint32_t f = ((sbase + s * P::STAGE + P::OFF_SFA) >> 4) + LO, c = tmem + P::SF_COL + (u & 1) * P::SF_SLOT;
+                const int nk = min(4, p.nks - 4 * kt);
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) {
+                        if (kk >= nk) break;
+                        cp_sf_pair(c + kk * 4 * (1 + P::NA), f + kk * (ATOM >> 4));
+#pragma unroll
+                        for (int a = 0; a < P::NA; a++)
+                            cp_sf_pair(c + kk * 4 * (1 + P::NA) + 4 + 4 * a, f + ((SFA_BYTES + a * SFA_BYTES + kk * ATOM) >> 4));
+                    }
+                    commit_one(&sf_full[u & 1]);
+                }
+                __syncwarp();
+                if (++s == S) s = 0, ph ^= 1;
+                if (++kt == p.nst) kt = 0;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------ epilogue: each CTA its 128 lanes
+        int t = 0;
+        for (int i = first; i < p.ntiles; i += step, t++) {
+            if (!all_wait(&acc_full[t & 1], (t >> 1) & 1, abort_flag, p.wait)) break;
+            tc_fence_after();
+            const int a = i % p.nba * 256 + rank * 128 + tid, b0 = i / p.nba * TN;
+            const uint32_t d = tmem + (t & 1) * P::ACC1 + ((uint32_t)(warp * 32) << 16);
+            const float sa = a < p.A ? p.sa[(int64_t)a * p.sa_step] : 0.f;
+            const bool in = a < p.A;
+            auto put = [&](int c0, const float(&v)[32]) {
+                const int left = p.B - b0 - c0;   // columns from here that exist
+                if (left <= 0) return;
+                const bool each = p.sb_step != 0;
+                const float sb = p.sb[each ? b0 + c0 + min(lane, left - 1) : 0];
+                if (p.tokens_on_lanes) {
+                    const int64_t at = (int64_t)a * p.N + b0 + c0;
+                    if (each) store_run<T, EPI>(p.y, p.res, at, in, left, v, sa, sb, true);
+                    else store_run<T, EPI>(p.y, p.res, at, in, left, v, sa, sb, false);
+                } else {
+                    store_columns<T, EPI>(p.y, p.res, (int64_t)(b0 + c0) * p.N + a, p.N, in, left, v, sb, sa);
+                }
+            };
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_remote(in_leader(&acc_free[t & 1]));
+            };
+            if constexpr (TN == 256) {
+                // the 96 columns shared with the other accumulator first (accumulator 0's last, 1's first)
+                const int c0 = t & 1 ? 0 : 160, c1 = t & 1 ? 96 : 0;
+                float v0[32], v1[32], v2[32];
+                tmem_ld32(d + c0, v0);
+                tmem_ld32(d + c0 + 32, v1);
+                tmem_ld32(d + c0 + 64, v2);
+                release();
+                put(c0, v0);
+                put(c0 + 32, v1);
+                put(c0 + 64, v2);
+#pragma unroll 1
+                for (int u = 0; u < 160; u += 32) {
+                    tmem_ld32(d + c1 + u, v0);
+                    put(c1 + u, v0);
+                }
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < TN; u += 32) {
+                    float v[32];
+                    tmem_ld32(d + u, v);
+                    if (u == TN - 32) release();
+                    put(u, v);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag && lane == 0) {
+        // As in gemm_kernel; a stage that only one CTA loaded never completes, and its wait ends by its bound, long
+        // after the copies have landed.
+        if (warp == 4 && rank == 0)
+            for (uint32_t u = q > (uint32_t)S ? q - S : 0; u < q; u++) mbar_wait(&full[u % S], (u / S) & 1);
+    }
+    if ((warp == 5 || warp == 6) && rank == 0 && *abort_flag) {   // the lane that issued: elect picks the same one
+        if (elect_one()) {
+            commit_one(drain);
+            mbar_wait(drain, 0);
+        }
+    }
+    __syncwarp();
+    cluster_sync();   // neither CTA leaves while the other may still signal it or run on its memory
+    if (warp == 5) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }
 
@@ -340,13 +734,72 @@ static int launch(Params p, const CUtensorMap &a, const uint8_t *x, int64_t byte
     return launch_status();
 }
 
+// Scale atoms as a 2-D u32 tensor [atoms][128], boxes of four (a stage's).
+static bool atom_map(CUtensorMap *m, const void *base, int64_t rows, int nks) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {ATOM / 4, (cuuint64_t)((rows + 127) / 128 * nks)};
+    const cuuint64_t strides[1] = {ATOM};
+    const cuuint32_t b[2] = {ATOM / 4, 4}, one[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int TN, typename T, int EPI>
+static int launch_pair(const Params &g, const uint8_t *w, const uint8_t *x, int64_t bytes, cudaStream_t st, int dev, const DeviceInfo &di) {
+    static std::atomic<uint64_t> done{0};
+    auto kern = pair_kernel<TN, T, EPI>;
+    PairParams p{};
+    // tokens on the lanes wherever y's rows allow 32-byte stores
+    p.tokens_on_lanes = (int64_t)g.N * sizeof(T) % 32 == 0 && !((reinterpret_cast<uintptr_t>(g.y) | reinterpret_cast<uintptr_t>(g.res)) & 31u);
+    const bool t = p.tokens_on_lanes;
+    p.sa = t ? g.sx : g.sw;
+    p.sb = t ? g.sw : g.sx;
+    p.sa_step = t ? g.sx_step : g.sw_step;
+    p.sb_step = t ? g.sw_step : g.sx_step;
+    p.A = t ? g.M : g.N;
+    p.B = t ? g.N : g.M;
+    p.nks = g.nks;
+    p.nst = g.nst;
+    p.nba = (p.A + 255) / 256;
+    p.ntiles = p.nba * ((p.B + TN - 1) / TN);
+    p.N = g.N;
+    p.res = g.res;
+    p.y = g.y;
+    p.wait = g.wait;
+    CUtensorMap a, b, sa, sb;
+    if (!code_map(&a, t ? x : w, p.A, bytes, 128) || !code_map(&b, t ? w : x, p.B, bytes, TN / 2) ||
+        !atom_map(&sa, t ? g.sfb : g.sfa, p.A, p.nks) || !atom_map(&sb, t ? g.sfa : g.sfb, p.B, p.nks))
+        return QMOE_ERR_LAUNCH;
+    if (!ensure_smem(kern, PairPlan<TN>::SMEM, dev, done)) return QMOE_ERR_LAUNCH;
+    cudaLaunchConfig_t cfg = {};
+    const int pairs = di.sms / 2;
+    cfg.gridDim = dim3((unsigned)(2 * (p.ntiles < pairs ? p.ntiles : pairs)));
+    cfg.blockDim = dim3(PAIR_THREADS);
+    cfg.dynamicSmemBytes = PairPlan<TN>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, p, a, b, sa, sb) != cudaSuccess) {
+        cudaGetLastError();
+        return QMOE_ERR_LAUNCH;
+    }
+    return launch_status();
+}
+
 template <typename T>
-static int pick(const Params &p, const CUtensorMap &a, const uint8_t *x, int64_t bytes, cudaStream_t st, int dev, const DeviceInfo &di) {
+static int pick(const Params &p, const CUtensorMap &a, const uint8_t *w, const uint8_t *x, int64_t bytes, cudaStream_t st, int dev, const DeviceInfo &di) {
     if (p.M <= 16) return launch<16, T>(p, a, x, bytes, st, dev, di);
     if (p.M <= 32) return launch<32, T>(p, a, x, bytes, st, dev, di);
     if (p.M <= 64) return launch<64, T>(p, a, x, bytes, st, dev, di);
     if (p.M <= 128 || (int64_t)p.nbn * ((p.M + 127) / 128) <= di.sms) return launch<128, T>(p, a, x, bytes, st, dev, di);
-    return launch<256, T>(p, a, x, bytes, st, dev, di);
+    if (p.epilogue == 0) return launch_pair<256, T, 0>(p, w, x, bytes, st, dev, di);
+    if (p.epilogue == 1) return launch_pair<256, T, 1>(p, w, x, bytes, st, dev, di);
+    return launch_pair<256, T, 2>(p, w, x, bytes, st, dev, di);
 }
 
 } // namespace g4
@@ -390,9 +843,9 @@ int dq_gemm_nvfp4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int
     CUtensorMap a;
     if (!g4::code_map(&a, w, N, K / 2, g4::BM)) return QMOE_ERR_LAUNCH;
     cudaStream_t st = as_stream(stream);
-    if (y_dtype == QMOE_DT_BF16) return g4::pick<__nv_bfloat16>(p, a, x, K / 2, st, dev, *di);
-    if (y_dtype == QMOE_DT_F16) return g4::pick<__half>(p, a, x, K / 2, st, dev, *di);
-    return g4::pick<float>(p, a, x, K / 2, st, dev, *di);
+    if (y_dtype == QMOE_DT_BF16) return g4::pick<__nv_bfloat16>(p, a, w, x, K / 2, st, dev, *di);
+    if (y_dtype == QMOE_DT_F16) return g4::pick<__half>(p, a, w, x, K / 2, st, dev, *di);
+    return g4::pick<float>(p, a, w, x, K / 2, st, dev, *di);
 }
 
 int dq_gemm_nvfp4_status(int clear, void *stream) {
