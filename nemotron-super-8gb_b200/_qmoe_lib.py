@@ -59,6 +59,8 @@ SIGNATURES = {
     "dq_scale_atoms": (_i, [_p, _i64, _i64, _p, _p]),
     "dq_dequant_nvfp4": (_i, [_p, _p, _p, _i, _i64, _i64, _i64, _i64, _p, _i, _p]),
     "dq_gemm_nvfp4": (_i, [_p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i, _p]),
+    "dq_linear_a4_workspace_bytes": (_sz, [_i64, _i64]),
+    "dq_linear_a4": (_i, [_p, _p, _p, _i, _p, _i, _i64, _i, _i, _i, _i, _p, _p, _p, _sz, _p]),
     "dq_gemm_nvfp4_status": (_i, [_i, _p]),
     "dq_dequant_rows": (_i, [_i, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i, _p]),
 }
@@ -100,8 +102,7 @@ def call(name, *args):
 
 def stream_of(t=None):
     """cudaStream_t of torch's current stream on the tensor's device."""
-    dev = t.device if t is not None else None
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.get_device() if t is not None else torch.cuda.current_device())
 
 
 def ptr(t):

@@ -706,7 +706,7 @@ static int launch(Params p, const CUtensorMap &a, const uint8_t *x, int64_t byte
     auto kern = gemm_kernel<TN, T>;
     CUtensorMap b;
     if (!code_map(&b, x, p.M, bytes, TN)) return QMOE_ERR_LAUNCH;
-    if (!ensure_smem(kern, P::SMEM, dev, done)) return QMOE_ERR_LAUNCH;
+    if (!(done.load(std::memory_order_acquire) >> (dev & 63) & 1) && !ensure_smem(kern, P::SMEM, dev, done)) return QMOE_ERR_LAUNCH;
     p.ntiles = p.nbn * ((p.M + TN - 1) / TN);
     p.split = 1;
     if constexpr (TN <= 128) {   // too few tiles for the SMs: a cluster per tile, each CTA an even part of the stages
@@ -771,7 +771,7 @@ static int launch_pair(const Params &g, const uint8_t *w, const uint8_t *x, int6
     if (!code_map(&a, t ? x : w, p.A, bytes, 128) || !code_map(&b, t ? w : x, p.B, bytes, TN / 2) ||
         !atom_map(&sa, t ? g.sfb : g.sfa, p.A, p.nks) || !atom_map(&sb, t ? g.sfa : g.sfb, p.B, p.nks))
         return QMOE_ERR_LAUNCH;
-    if (!ensure_smem(kern, PairPlan<TN>::SMEM, dev, done)) return QMOE_ERR_LAUNCH;
+    if (!(done.load(std::memory_order_acquire) >> (dev & 63) & 1) && !ensure_smem(kern, PairPlan<TN>::SMEM, dev, done)) return QMOE_ERR_LAUNCH;
     cudaLaunchConfig_t cfg = {};
     const int pairs = di.sms / 2;
     cfg.gridDim = dim3((unsigned)(2 * (p.ntiles < pairs ? p.ntiles : pairs)));
@@ -846,6 +846,25 @@ int dq_gemm_nvfp4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int
     if (y_dtype == QMOE_DT_BF16) return g4::pick<__nv_bfloat16>(p, a, w, x, K / 2, st, dev, *di);
     if (y_dtype == QMOE_DT_F16) return g4::pick<__half>(p, a, w, x, K / 2, st, dev, *di);
     return g4::pick<float>(p, a, w, x, K / 2, st, dev, *di);
+}
+
+size_t dq_linear_a4_workspace_bytes(int64_t M, int64_t K) {
+    if (M < 1 || M > (1 << 24) || K < 32 || (K % 32) || K > (1 << 24)) return 0;
+    return (size_t)(M * (K / 2) + (M + 127) / 128 * ((K + 63) / 64) * g4::ATOM + (M + 3) / 4 * 16 + M * (K / 16));
+}
+
+int dq_linear_a4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int sw_per_row, const void *x, int x_dtype,
+                 int64_t ldx, int M, int N, int K, int epilogue, const void *residual, void *y, void *workspace,
+                 size_t workspace_bytes, void *stream) {
+    if (!w || !w_atoms || !sw || !x || !y || !workspace || (epilogue == 2 && !residual)) return QMOE_ERR_NULL;
+    const size_t need = dq_linear_a4_workspace_bytes(M, K);
+    if (!need || N < 1 || N > (1 << 24) || epilogue < 0 || epilogue > 2) return QMOE_ERR_SHAPE;
+    if (!aligned16(workspace)) return QMOE_ERR_ALIGN;
+    if (workspace_bytes < need) return QMOE_ERR_WORKSPACE;
+    uint8_t *codes = static_cast<uint8_t *>(workspace), *atoms = codes + (int64_t)M * (K / 2);
+    uint8_t *s = atoms + (int64_t)((M + 127) / 128) * ((K + 63) / 64) * g4::ATOM, *sc = s + (int64_t)(M + 3) / 4 * 16;
+    if (int e = dq_quantize_nvfp4(x, x_dtype, ldx, M, K, 1, codes, sc, reinterpret_cast<float *>(s), atoms, stream)) return e;
+    return dq_gemm_nvfp4(w, w_atoms, sw, sw_per_row, codes, atoms, reinterpret_cast<float *>(s), 1, M, N, K, epilogue, residual, y, x_dtype, stream);
 }
 
 int dq_gemm_nvfp4_status(int clear, void *stream) {

@@ -17,7 +17,8 @@ namespace qmoe {
 namespace qz {
 
 constexpr int THREADS = 256;
-constexpr int KEEP = 4;   // 16-element blocks a thread keeps in registers between the row maximum and the codes
+// 16-element blocks a thread keeps in registers between the row maximum and the codes: 64 registers of elements
+template <typename T> constexpr int KEEP = sizeof(T) == 4 ? 4 : 8;
 
 // 16 consecutive elements as loaded.
 template <typename T> struct Raw { uint32_t r[sizeof(T) * 4]; };
@@ -112,6 +113,7 @@ struct Args {
     int64_t M;
     int nb;        // blocks per row, K / 16
     int vec;       // rows are 16-byte aligned
+    int words;     // whole k-steps per row: four scales are one aligned word
     uint8_t *w, *sc, *atoms;
     float *s;      // per row: written; per tensor: read
 };
@@ -125,21 +127,23 @@ __device__ __forceinline__ int64_t atom_at(int64_t r, int ks, int nks) {
 // Stores a block's codes and scale, and the k-step's four scales as one word of the atoms (b runs over whole k-steps;
 // blocks at or past nb are padding with scale zero).
 __device__ __forceinline__ void put(const Args &a, int64_t row, int b, bool live, uint2 codes, uint32_t sb) {
-    if (live) {
-        *reinterpret_cast<uint2 *>(a.w + (row * a.nb + b) * 8) = codes;
+    if (live) *reinterpret_cast<uint2 *>(a.w + (row * a.nb + b) * 8) = codes;
+    uint32_t v = live ? sb : 0u;
+    v |= __shfl_down_sync(0xffffffffu, v, 1) << 8;
+    v |= __shfl_down_sync(0xffffffffu, v, 2) << 16;
+    const int nks = (a.nb + 3) >> 2;
+    const bool first = !(b & 3) && (b >> 2) < nks;
+    if (a.words) {
+        if (first) *reinterpret_cast<uint32_t *>(a.sc + row * a.nb + b) = v;
+    } else if (live) {
         a.sc[row * a.nb + b] = (uint8_t)sb;
     }
-    if (a.atoms) {
-        uint32_t v = live ? sb : 0u;
-        v |= __shfl_down_sync(0xffffffffu, v, 1) << 8;
-        v |= __shfl_down_sync(0xffffffffu, v, 2) << 16;
-        const int nks = (a.nb + 3) >> 2;
-        if (!(b & 3) && (b >> 2) < nks) *reinterpret_cast<uint32_t *>(a.atoms + atom_at(row, b >> 2, nks)) = v;
-    }
+    if (a.atoms && first) *reinterpret_cast<uint32_t *>(a.atoms + atom_at(row, b >> 2, nks)) = v;
 }
 
-// One row per G threads (32: a warp, so that short rows do not wait for a whole CTA; 256: a CTA). The row's blocks stay
-// in registers between the maximum and the codes, up to KEEP a thread; longer rows are read again (from L2).
+// One row per G threads. G = 32, a warp: no barrier between the row's maximum and its codes, and 16 wide loads of 128 B
+// in flight per lane (16384 x 4096 bf16: 66 us with a CTA per row). G = 256, a CTA, for rows that a warp cannot keep and
+// for so few rows that warps would leave SMs idle. Blocks past the KEEP a thread keeps are read again (from L2).
 template <typename T, int G>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a) {
     __shared__ uint32_t red[THREADS / 32];
@@ -147,20 +151,20 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a) {
     const int64_t row = blockIdx.x * (int64_t)(THREADS / G) + threadIdx.x / G;
     const bool in = row < a.M;   // a warp is all in or all out
     const T *x = static_cast<const T *>(a.x) + (in ? row : 0) * a.ldx;
-    Raw<T> keep[KEEP];
+    Raw<T> keep[KEEP<T>];
     uint32_t m = 0;
     if (in) {
 #pragma unroll
-        for (int i = 0; i < KEEP; i++)
+        for (int i = 0; i < KEEP<T>; i++)
             if (t + i * G < a.nb) load16(x + (t + i * G) * 16, a.vec, keep[i]);
 #pragma unroll
-        for (int i = 0; i < KEEP; i++)
+        for (int i = 0; i < KEEP<T>; i++)
             if (t + i * G < a.nb) {
                 float f[16];
                 widen(keep[i], f);
                 m = max(m, amax_bits(f));
             }
-        for (int b = t + KEEP * G; b < a.nb; b += G) {
+        for (int b = t + KEEP<T> * G; b < a.nb; b += G) {
             Raw<T> v;
             float f[16];
             load16(x + (int64_t)b * 16, a.vec, v);
@@ -181,7 +185,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a) {
     if (t == 0) a.s[row] = pow2f(e);
     const int lim = (a.nb + 31) & ~31;   // whole warps, for the shuffles of put()
 #pragma unroll
-    for (int i = 0; i < KEEP; i++) {
+    for (int i = 0; i < KEEP<T>; i++) {
         const int b = t + i * G;
         if (b < lim) {
             uint2 c = make_uint2(0u, 0u);
@@ -190,7 +194,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a) {
             put(a, row, b, b < a.nb, c, sb);
         }
     }
-    for (int b = t + KEEP * G; b < lim; b += G) {
+    for (int b = t + KEEP<T> * G; b < lim; b += G) {
         uint2 c = make_uint2(0u, 0u);
         uint32_t sb = 0;
         if (b < a.nb) {
@@ -232,7 +236,8 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) tensor_kernel(const Args a) {
     const float inv_s = pow2f(127 - (int)(__float_as_uint(*a.s) >> 23));
     const int lim = (a.nb + 31) & ~31;
-    for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
+    for (int64_t i = blockIdx.y; i < a.M; i += gridDim.y) {
+        const int64_t row = a.M - 1 - i;   // the first pass ended with the last rows: L2 still holds those
         const T *x = static_cast<const T *>(a.x) + row * a.ldx;
         for (int b = blockIdx.x * THREADS + threadIdx.x; b < lim; b += gridDim.x * THREADS) {
             uint2 c = make_uint2(0u, 0u);
@@ -248,9 +253,9 @@ __global__ void __launch_bounds__(THREADS) tensor_kernel(const Args a) {
 }
 
 template <typename T>
-static int launch(const Args &a, bool per_row, cudaStream_t st) {
+static int launch(const Args &a, bool per_row, cudaStream_t st, const DeviceInfo &di) {
     if (per_row) {
-        if (a.nb <= 32 * KEEP) {
+        if (a.nb <= 32 || (a.nb <= 32 * KEEP<T> && a.M >= 8 * di.sms)) {
             const int64_t g = (a.M + THREADS / 32 - 1) / (THREADS / 32);
             rows_kernel<T, 32><<<(unsigned)g, THREADS, 0, st>>>(a);
         } else {
@@ -261,7 +266,7 @@ static int launch(const Args &a, bool per_row, cudaStream_t st) {
     if (cudaMemsetAsync(a.s, 0, sizeof(float), st) != cudaSuccess) return QMOE_ERR_LAUNCH;
     const unsigned gx = (unsigned)((a.nb + THREADS - 1) / THREADS);
     const dim3 grid(gx, (unsigned)(a.M < 32768 ? a.M : 32768));
-    const unsigned scan = 148 * 8 / gx > 0 ? 148 * 8 / gx : 1;
+    const unsigned scan = di.sms * 8 / gx > 0 ? di.sms * 8 / gx : 1;
     tensor_scale_kernel<T><<<dim3(gx, a.M < scan ? (unsigned)a.M : scan), THREADS, 0, st>>>(a);
     tensor_kernel<T><<<grid, THREADS, 0, st>>>(a);
     return launch_status();
@@ -347,21 +352,23 @@ int dq_quantize_nvfp4(const void *x, int x_dtype, int64_t ldx, int64_t M, int64_
     const int size = x_dtype == QMOE_DT_F32 ? 4 : 2;
     if ((reinterpret_cast<uintptr_t>(x) % size) || (reinterpret_cast<uintptr_t>(w) & 7u) || !aligned4(s) || !aligned4(atoms))
         return QMOE_ERR_ALIGN;
-    if (int e = current_device(nullptr, nullptr)) return e;
+    DeviceInfo *di;
+    if (int e = current_device(nullptr, &di)) return e;
     qz::Args a{};
     a.x = x;
     a.ldx = ldx;
     a.M = M;
     a.nb = (int)(K / 16);
     a.vec = aligned16(x) && (ldx * size) % 16 == 0;
+    a.words = a.nb % 4 == 0 && aligned4(sc);
     a.w = w;
     a.sc = sc;
     a.s = s;
     a.atoms = atoms;
     cudaStream_t st = as_stream(stream);
-    if (x_dtype == QMOE_DT_BF16) return qz::launch<__nv_bfloat16>(a, per_row != 0, st);
-    if (x_dtype == QMOE_DT_F16) return qz::launch<__half>(a, per_row != 0, st);
-    return qz::launch<float>(a, per_row != 0, st);
+    if (x_dtype == QMOE_DT_BF16) return qz::launch<__nv_bfloat16>(a, per_row != 0, st, *di);
+    if (x_dtype == QMOE_DT_F16) return qz::launch<__half>(a, per_row != 0, st, *di);
+    return qz::launch<float>(a, per_row != 0, st, *di);
 }
 
 int dq_scale_atoms(const uint8_t *sc, int64_t N, int64_t K, uint8_t *atoms, void *stream) {

@@ -139,12 +139,13 @@ def attach(lin, q):
 
 class _on:
     """The tensor's device as the current one, for the launch (nothing to do where it is)."""
+    __slots__ = ("dev", "was")
 
     def __init__(self, t):
-        self.dev = t.device.index if t.is_cuda else None
+        self.dev = t.get_device()
 
     def __enter__(self):
-        self.was = torch.cuda.current_device() if self.dev is not None else None
+        self.was = torch._C._cuda_getDevice()
         if self.was != self.dev:
             torch.cuda.set_device(self.dev)
 
@@ -162,13 +163,23 @@ def _no_grad(*ts):
         raise C.QmoeError("the four-bit operators have no gradient: call them under torch.no_grad()")
 
 
+def _rows(x):
+    """A matrix as the kernels read it: unit column stride, rows that do not overlap; its dtype code and row stride."""
+    _no_grad(x)
+    C.ptr(x)
+    dt = C.dtype_code(x)
+    M, K = x.shape
+    if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
+        x = x.contiguous()
+    return x, dt, x.stride(0) if M > 1 else K
+
+
 def quantize(x, per_row=True):
     """x [M, K] (bf16, fp16 or fp32; K a multiple of 16; rows may be strided) -> quantized dict: codes "w" [M, K/2],
     block scales "sc" [M, K/16] (e4m3 bytes), "s" f32 [M] with fmt "nvfp4_rows" (per_row), or [1] with fmt "nvfp4"
     (one scale for the tensor: a weight of this module), and "sca", the scales as gemm reads them. s is the smallest
     power of two with amax <= 2688 s, scales and codes the nearest, ties to even. A 16-element block that holds an
     infinity or a NaN reads back as NaN; the others are as if that value were zero."""
-    _no_grad(x)
     if x.dim() != 2:
         raise C.QmoeError("quantize takes a matrix [M, K]")
     M, K = x.shape
@@ -176,10 +187,7 @@ def quantize(x, per_row=True):
         raise C.QmoeError(f"quantize takes rows of a positive multiple of 16 elements (got {K})")
     if M == 0 and not per_row:
         raise C.QmoeError("a tensor without rows has no scale")
-    C.ptr(x)
-    dt = C.dtype_code(x)
-    if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
-        x = x.contiguous()
+    x, dt, ld = _rows(x)
     dev = x.device
     q = {"fmt": "nvfp4_rows" if per_row else "nvfp4", "w": torch.empty(M, K // 2, dtype=torch.uint8, device=dev),
          "sc": torch.empty(M, K // 16, dtype=torch.uint8, device=dev),
@@ -187,8 +195,8 @@ def quantize(x, per_row=True):
          "sca": torch.empty(_atoms_bytes(M, K), dtype=torch.uint8, device=dev)}
     if M:
         with _on(x):
-            C.call("dq_quantize_nvfp4", C.ptr(x), dt, int(x.stride(0)) if M > 1 else K, M, K, int(per_row),
-                   C.ptr(q["w"]), C.ptr(q["sc"]), C.ptr(q["s"]), C.ptr(q["sca"]), C.stream_of(x))
+            C.call("dq_quantize_nvfp4", x.data_ptr(), dt, ld, M, K, int(per_row), q["w"].data_ptr(), q["sc"].data_ptr(),
+                   q["s"].data_ptr(), q["sca"].data_ptr(), C.stream_of(x))
     return q
 
 
@@ -208,53 +216,73 @@ def prepare(q):
 
 
 _ACTS = {None: 0, "relu2": 1}
+_NVFP4 = ("nvfp4", "nvfp4_rows")
+
+
+def _check_product(q, M, K, dtype, dev, act, residual):
+    """The epilogue's code, and the residual as the kernels read it."""
+    if q["fmt"] not in _NVFP4:
+        raise C.QmoeError(f"gemm takes NVFP4 operands (got {q['fmt']})")
+    if q["K"] != K:
+        raise C.QmoeError(f"gemm: {K} elements per activation row, {q['K']} per weight row")
+    if K % 32 or K == 0:
+        raise C.QmoeError(f"gemm takes rows of a positive multiple of 32 elements (got {K})")
+    if act not in _ACTS or (act is not None and residual is not None):
+        raise C.QmoeError("gemm: act is None or 'relu2', and not together with a residual")
+    if dtype not in C.DT:
+        raise C.QmoeError(f"unsupported output dtype {dtype}")
+    if q["w"].device != dev:
+        raise C.QmoeError(f"gemm: weight on {q['w'].device}, activations on {dev}")
+    if residual is None:
+        return _ACTS[act], None
+    _no_grad(residual)
+    if residual.shape != (M, q["N"]) or residual.dtype != dtype or residual.device != dev:
+        raise C.QmoeError("gemm: the residual is [M, N] in the output's dtype, on its device")
+    return 2, residual.contiguous()
 
 
 def gemm(q, xq, dtype=torch.bfloat16, act=None, residual=None):
     """y [M, N] in dtype = dequant(xq) @ dequant(q).T for two NVFP4 dicts (xq of quantize: activations; q: a weight,
     best one that went through prepare, else its scales are laid out in this call), products exact, fp32 sums in a
     fixed order. act "relu2": relu(y)^2; residual [M, N] in dtype: y + residual; each on y rounded to dtype, as the
-    unfused torch operators. K a multiple of 32; rows without elements are refused."""
-    for d in (q, xq):
-        if d["fmt"] not in ("nvfp4", "nvfp4_rows"):
-            raise C.QmoeError(f"gemm takes NVFP4 operands (got {d['fmt']})")
-    M, N, K = xq["N"], q["N"], q["K"]
-    if xq["K"] != K:
-        raise C.QmoeError(f"gemm: {xq['K']} elements per activation row, {K} per weight row")
-    if K % 32:
-        raise C.QmoeError(f"gemm takes rows of a multiple of 32 elements (got {K})")
-    if act not in _ACTS or (act is not None and residual is not None):
-        raise C.QmoeError("gemm: act is None or 'relu2', and not together with a residual")
-    if dtype not in C.DT:
-        raise C.QmoeError(f"unsupported output dtype {dtype}")
+    unfused torch operators. K a multiple of 32."""
+    if xq["fmt"] not in _NVFP4:
+        raise C.QmoeError(f"gemm takes NVFP4 operands (got {xq['fmt']})")
+    M, N, K = xq["N"], q["N"], xq["K"]
     dev = xq["w"].device
-    if q["w"].device != dev:
-        raise C.QmoeError(f"gemm: weight on {q['w'].device}, activations on {dev}")
-    if residual is not None:
-        _no_grad(residual)
-        if residual.shape != (M, N) or residual.dtype != dtype or residual.device != dev:
-            raise C.QmoeError("gemm: the residual is [M, N] in the output's dtype, on its device")
-        residual = residual.contiguous()
+    ep, residual = _check_product(q, M, K, dtype, dev, act, residual)
     y = torch.empty(M, N, dtype=dtype, device=dev)
     if M == 0 or N == 0:
         return y
     q, xq = prepare(q), prepare(xq)
     with _on(y):
         C.call("dq_gemm_nvfp4", C.ptr(q["w"]), C.ptr(q["sca"]), C.ptr(q["s"]), int(q["fmt"] == "nvfp4_rows"),
-               C.ptr(xq["w"]), C.ptr(xq["sca"]), C.ptr(xq["s"]), int(xq["fmt"] == "nvfp4_rows"), M, N, K,
-               2 if residual is not None else _ACTS[act], C.ptr(residual), C.ptr(y), C.DT[dtype], C.stream_of(y))
+               C.ptr(xq["w"]), C.ptr(xq["sca"]), C.ptr(xq["s"]), int(xq["fmt"] == "nvfp4_rows"), M, N, K, ep,
+               C.ptr(residual), C.ptr(y), C.DT[dtype], C.stream_of(y))
     return y
 
 
 def qlinear_a4(q, x, act=None, residual=None):
-    """qlinear with the activations in NVFP4 too: x [..., K] is quantized row by row, then gemm: [..., N] in x.dtype.
-    The result carries the activations' four-bit rounding (about a tenth of a row's norm), for half or less of the
-    time of a bf16 product."""
+    """qlinear with the activations in NVFP4 too: x [..., K] is quantized row by row, then multiplied as gemm does:
+    [..., N] in x.dtype (residual of that shape). The result carries the activations' four-bit rounding (about a tenth
+    of a row's norm) and takes a fraction of a bf16 product's time."""
     sh = x.shape
-    x2 = x.reshape(-1, sh[-1])
+    K, N = sh[-1], q["N"]
+    x, dt, ld = _rows(x if len(sh) == 2 else x.reshape(-1, K))
+    M, dev = x.shape[0], x.device
     if residual is not None:
-        residual = residual.reshape(-1, q["N"])
-    return gemm(q, quantize(x2), x.dtype, act, residual).view(*sh[:-1], q["N"])
+        residual = residual.reshape(-1, N)
+    ep, residual = _check_product(q, M, K, x.dtype, dev, act, residual)
+    y = torch.empty(M, N, dtype=x.dtype, device=dev)
+    if M and N:
+        q = prepare(q)
+        n = M * (K // 2) + _atoms_bytes(M, K) + (M + 3) // 4 * 16 + M * (K // 16)   # dq_linear_a4_workspace_bytes
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        with _on(x):
+            C.call("dq_linear_a4", q["w"].data_ptr(), q["sca"].data_ptr(), q["s"].data_ptr(), int(q["fmt"] == "nvfp4_rows"),
+                   x.data_ptr(), dt, ld, M, N, K, ep, residual.data_ptr() if residual is not None else None, y.data_ptr(),
+                   ws.data_ptr(), n, C.stream_of(x))
+    return y if len(sh) == 2 else y.view(*sh[:-1], N)
 
 
 def gemm_status(device=None, clear=True):

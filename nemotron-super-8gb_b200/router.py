@@ -5,6 +5,8 @@ expert: the same experts and weights, in decreasing order of choice, ties to the
 gradient to the logits (the choice itself has none; `bias` gets none, it is moved by the counts). `balance_loss` is the
 auxiliary loss that keeps the experts evenly loaded, with its gradient. Both take CUDA tensors only.
 """
+import functools
+
 import torch
 
 import _qmoe_lib as C
@@ -31,20 +33,26 @@ def _rows(x):
     return x, int(x.stride(0)) if x.shape[0] > 1 else x.shape[1]
 
 
+def _route(x, bias, top_k, scaling, n_group, topk_group, norm, score):
+    x, ld = _rows(x)
+    T, E = x.shape
+    dev = x.device
+    ids = torch.empty(T, top_k, dtype=torch.int64, device=dev)
+    w = torch.empty(T, top_k, dtype=torch.float32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev) if T else torch.zeros(E, dtype=torch.int32, device=dev)
+    if T:
+        with _on(x):
+            C.call("qmoe_route", x.data_ptr(), C.DT[x.dtype], ld, bias.data_ptr() if bias is not None else None, T, E, top_k,
+                   n_group, topk_group, norm, score, scaling, ids.data_ptr(), w.data_ptr(), counts.data_ptr(), C.stream_of(x))
+    return ids, w, counts
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, top_k, scaling, n_group, topk_group, norm, score):
-        x, ld = _rows(logits)
-        T, E = x.shape
-        ids = torch.empty(T, top_k, dtype=torch.int64, device=x.device)
-        w = torch.empty(T, top_k, dtype=torch.float32, device=x.device)
-        counts = torch.empty(E, dtype=torch.int32, device=x.device) if T else torch.zeros(E, dtype=torch.int32, device=x.device)
-        if T:
-            with _on(x):
-                C.call("qmoe_route", C.ptr(x), C.dtype_code(x), ld, C.ptr(bias), T, E, top_k, n_group, topk_group, norm, score,
-                       scaling, C.ptr(ids), C.ptr(w), C.ptr(counts), C.stream_of(x))
+    def forward(ctx, logits, *args):
+        ids, w, counts = _route(logits, *args)
         ctx.save_for_backward(logits, ids)
-        ctx.args = (top_k, norm, score, scaling)
+        ctx.args = args[1:]
         ctx.mark_non_differentiable(ids, counts)
         ctx.set_materialize_grads(False)
         return ids, w, counts
@@ -55,14 +63,14 @@ class _Route(torch.autograd.Function):
         if dw is None:
             return (None,) * 8
         logits, ids = ctx.saved_tensors
-        top_k, norm, score, scaling = ctx.args
+        top_k, scaling, _, _, norm, score = ctx.args
         x, ld = _rows(logits)
         dl = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         if x.shape[0]:
             dw = dw.to(torch.float32).contiguous()
             with _on(x):
-                C.call("qmoe_route_backward", C.ptr(x), C.dtype_code(x), ld, x.shape[0], x.shape[1], top_k, norm, score, scaling,
-                       C.ptr(ids), C.ptr(dw), C.ptr(dl), C.stream_of(x))
+                C.call("qmoe_route_backward", x.data_ptr(), C.DT[x.dtype], ld, x.shape[0], x.shape[1], top_k, norm, score, scaling,
+                       ids.data_ptr(), C.ptr(dw), dl.data_ptr(), C.stream_of(x))
         return (dl,) + (None,) * 7
 
 
@@ -85,26 +93,37 @@ def route(logits, bias=None, top_k=22, scaling=5.0, n_group=1, topk_group=1, nor
         if bias.shape != (E,) or bias.device != logits.device:
             raise C.QmoeError("bias must be [E], on the logits' device")
         bias = bias.detach().to(torch.float32).contiguous()
-    return _Route.apply(logits, bias, int(top_k), float(scaling), int(n_group), int(topk_group), int(bool(norm_topk_prob)),
-                        _SCORES[score])
+    args = (bias, int(top_k), float(scaling), int(n_group), int(topk_group), int(bool(norm_topk_prob)), _SCORES[score])
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Route.apply(logits, *args)
+    return _route(logits, *args)
+
+
+_bytes = functools.lru_cache(maxsize=256)(lambda T, E: int(C.lib().qmoe_balance_workspace_bytes(T, E)))
+
+
+def _balance(x, ids, mask, score, coef):
+    """Loss, counts, and coef * f / T' per expert for the backward pass."""
+    x, ld = _rows(x)
+    T, E = x.shape
+    dev = x.device
+    if T == 0:
+        return torch.zeros((), device=dev), torch.zeros(E, dtype=torch.int32, device=dev), torch.zeros(E, device=dev)
+    loss, counts = torch.empty((), dtype=torch.float32, device=dev), torch.empty(E, dtype=torch.int32, device=dev)
+    c = torch.empty(E, dtype=torch.float32, device=dev)
+    n = _bytes(T, E)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    with _on(x):
+        C.call("qmoe_balance", x.data_ptr(), C.DT[x.dtype], ld, ids.data_ptr(), int(ids.dtype == torch.int64),
+               mask.data_ptr() if mask is not None else None, T, E, ids.shape[1], score, coef, loss.data_ptr(), counts.data_ptr(),
+               c.data_ptr(), ws.data_ptr(), n, C.stream_of(x))
+    return loss, counts, c
 
 
 class _Balance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, mask, score, coef):
-        x, ld = _rows(logits)
-        T, E = x.shape
-        dev = x.device
-        if T == 0:
-            loss, counts = torch.zeros((), device=dev), torch.zeros(E, dtype=torch.int32, device=dev)
-            c = torch.zeros(E, device=dev)
-        else:
-            loss, counts = torch.empty((), device=dev), torch.empty(E, dtype=torch.int32, device=dev)
-            c = torch.empty(E, device=dev)
-            ws = torch.empty(int(C.lib().qmoe_balance_workspace_bytes(T, E)), dtype=torch.uint8, device=dev)
-            with _on(x):
-                C.call("qmoe_balance", C.ptr(x), C.dtype_code(x), ld, C.ptr(ids), int(ids.dtype == torch.int64), C.ptr(mask), T, E,
-                       ids.shape[1], score, coef, C.ptr(loss), C.ptr(counts), C.ptr(c), C.ptr(ws), ws.numel(), C.stream_of(x))
+        loss, counts, c = _balance(logits, ids, mask, score, coef)
         ctx.save_for_backward(logits, mask, c)
         ctx.score = score
         ctx.mark_non_differentiable(counts)
@@ -120,10 +139,10 @@ class _Balance(torch.autograd.Function):
         x, ld = _rows(logits)
         dl = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         if x.shape[0]:
-            g = dloss.to(torch.float32).contiguous()
+            g = dloss.to(torch.float32)
             with _on(x):
-                C.call("qmoe_balance_backward", C.ptr(x), C.dtype_code(x), ld, C.ptr(mask), x.shape[0], x.shape[1], ctx.score,
-                       C.ptr(c), C.ptr(g), C.ptr(dl), C.stream_of(x))
+                C.call("qmoe_balance_backward", x.data_ptr(), C.DT[x.dtype], ld, mask.data_ptr() if mask is not None else None,
+                       x.shape[0], x.shape[1], ctx.score, c.data_ptr(), C.ptr(g), dl.data_ptr(), C.stream_of(x))
         return dl, None, None, None, None
 
 
@@ -143,4 +162,7 @@ def balance_loss(logits, ids, mask=None, score="sigmoid", coef=1.0):
         if mask.shape != (T,) or mask.dtype != torch.bool or mask.device != logits.device:
             raise C.QmoeError("mask must be bool [T], on the logits' device")
         mask = mask.contiguous()
-    return _Balance.apply(logits, ids.contiguous(), mask, _SCORES[score], float(coef))
+    args = (ids.contiguous(), mask, _SCORES[score], float(coef))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Balance.apply(logits, *args)
+    return _balance(logits, *args)[:2]
