@@ -5,11 +5,18 @@
 //   sc = e4m3(amax16 / (6 s)), nearest, ties to even,
 //   q  = e2m1(x / (s sc)), nearest, ties to even; value = q * sc * s.
 // A power of two loses nothing against s = amax / 2688: the block scale is itself a floating-point number, and
-// x / s is then exact. Every decision is the exact one: what is compared is x / s against 6 * midpoint or midpoint *
-// sc, numbers of at most 7 significant bits, so an fp32 x may first be cut to 13 bits with the rest ORed into the
-// last ("round to odd"), and x / s * (1 / sc), off by under 2^-22, is rounded to 18 bits before the conversion,
-// which puts exact ties back on the tie and moves nothing else across (the nearest other value is 2^-12 away).
-// A block that holds an infinity or a NaN gets the scale NaN (0x7F) and zero codes; s ignores those elements.
+// x / s is then exact. A block that holds an infinity or a NaN gets the scale NaN (0x7F) and zero codes; s ignores
+// those elements.
+//
+// Every decision is the exact one, without a division. What is compared is x / s with midpoint * sc, or amax16 / s with
+// 6 * midpoint: numbers of at most 7 significant bits. An fp32 x is first cut to 13 bits with the rest ORed into the last
+// ("round to odd"), which keeps its order among such numbers; bf16 and f16 have fewer anyway. So a quotient that is no
+// tie is at least 2^-12 of its size away from one. x * (1 / (s sc)) + 192 in one FMA rounds the quotient (at most 6.5, its
+// reciprocal off by 2^-23) to a multiple of 2^-16: a tie comes back as the tie, and nothing else reaches one, the smallest
+// distance being 0.25 * 2^-12. amax16 / 6 is rounded to 18 bits to the same end.
+//
+// Bounds: bytes (2.56 an element for bf16) and next to them issue, about 7 instructions an element; with IEEE divisions
+// and per-element comparisons it was 16, and 16384 x 4096 bf16 took 61 us.
 #include "common.cuh"
 #include "host.h"
 
@@ -17,8 +24,7 @@ namespace qmoe {
 namespace qz {
 
 constexpr int THREADS = 256;
-// 16-element blocks a thread keeps in registers between the row maximum and the codes: 64 registers of elements
-template <typename T> constexpr int KEEP = sizeof(T) == 4 ? 4 : 8;
+constexpr int KEEP = 4;   // 16-element blocks a thread keeps in registers between the row maximum and the codes
 
 // 16 consecutive elements as loaded.
 template <typename T> struct Raw { uint32_t r[sizeof(T) * 4]; };
@@ -54,15 +60,29 @@ template <typename T> __device__ __forceinline__ void widen(const Raw<T> &v, flo
     }
 }
 
-// Bits of the largest finite magnitude of a block.
-__device__ __forceinline__ uint32_t amax_bits(const float (&f)[16]) {
+// fp32 bits of the largest finite magnitude of a block; with NONFINITE set where the block holds anything else.
+constexpr uint32_t NONFINITE = 0x80000000u;
+template <typename T> __device__ __forceinline__ uint32_t block_max(const Raw<T> &v) {
     uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
+        for (int i = 0; i < 16; i++) m = max(m, v.r[i] & 0x7FFFFFFFu);
+        if (m < 0x7F800000u) return m;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = __vmaxu2(m, v.r[i] & 0x7FFF7FFFu);
+        m = max(m & 0xFFFFu, m >> 16);
+        if (std::is_same<T, __half>::value && m < 0x7C00u) return __float_as_uint(__half2float(__ushort_as_half((uint16_t)m)));
+        if (!std::is_same<T, __half>::value && m < 0x7F80u) return m << 16;
+    }
+    float f[16];
+    widen(v, f);
+    m = 0;
     for (int i = 0; i < 16; i++) {
         const uint32_t b = __float_as_uint(f[i]) & 0x7FFFFFFFu;
         m = max(m, b >= 0x7F800000u ? 0u : b);
     }
-    return m;
+    return m | NONFINITE;
 }
 
 // Exponent e of s = 2^e for a largest magnitude with these bits: 2688 = 1.3125 * 2^11.
@@ -71,38 +91,42 @@ __device__ __forceinline__ int scale_exp(uint32_t bits) {
     return max(e, -126);
 }
 
-// One block: codes (element 2i in the low nibble of byte i) and scale byte, for u = x * 2^-e.
-template <typename T>
-__device__ __forceinline__ uint32_t block16(const Raw<T> &v, float inv_s, uint2 &codes) {
-    float u[16];
-    widen(v, u);
-    uint32_t top = 0;
+// Round to odd at 13 significant bits (of a normal number's bits).
+__device__ __forceinline__ uint32_t odd13(uint32_t b) { return (b | ((b & 0x7FFu) + 0x7FFu)) & ~0x7FFu; }
+
+// One block whose block_max is `top`: codes (element 2i in the low nibble of byte i) and scale byte, s = 2^e.
+template <typename T> __device__ __forceinline__ uint32_t block16(const Raw<T> &v, uint32_t top, int e, uint2 &codes) {
+    codes = make_uint2(0u, 0u);
+    if (top & NONFINITE) return 0x7Fu;
+    const float inv_s = pow2f(-e);
+    uint32_t m = __float_as_uint(__uint_as_float(top) * inv_s);
+    if constexpr (sizeof(T) == 4) m = odd13(m);
+    m = (__float_as_uint(__uint_as_float(m) * (1.f / 6.f)) + 0x20u) & ~0x3Fu;
+    uint32_t sb;
+    asm("{\n\t.reg .b16 t;\n\tcvt.rn.satfinite.e4m3x2.f32 t, %1, %2;\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(sb) : "f"(0.f), "f"(__uint_as_float(m)));
+    sb &= 0xFFu;
+    if (sb == 0u) return 0u;
+    float f, pre = 1.f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(e4m3_f32((uint8_t)sb)));
+    if (e >= -116) f *= inv_s;   // one factor for x / (s sc), off by the reciprocal's error alone
+    else pre = inv_s;            // rows of almost nothing: it would overflow
+    float q[16];
+    widen(v, q);
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-        u[i] *= inv_s;
-        if constexpr (sizeof(T) == 4) {   // round to odd at 13 bits (see above); infinities stay, a NaN stays a NaN
-            const uint32_t b = __float_as_uint(u[i]);
-            u[i] = __uint_as_float((b & ~0x7FFu) | ((b & 0x7FFu) ? 0x800u : 0u));
-        }
-        top = max(top, __float_as_uint(u[i]) & 0x7FFFFFFFu);
+        if (e < -116) q[i] *= pre;
+        if constexpr (sizeof(T) == 4) q[i] = __uint_as_float(odd13(__float_as_uint(q[i])));
+        q[i] = fmaf(q[i], f, 192.f) - 192.f;
     }
-    codes = make_uint2(0u, 0u);
-    if (top >= 0x7F800000u) return 0x7Fu;
-    uint32_t sb;
-    asm("{\n\t.reg .b16 t;\n\tcvt.rn.satfinite.e4m3x2.f32 t, %1, %2;\n\tcvt.u32.u16 %0, t;\n\t}"
-        : "=r"(sb) : "f"(0.f), "f"(__fdiv_rn(__uint_as_float(top), 6.f)));
-    sb &= 0xFFu;
-    const float d = e4m3_f32((uint8_t)sb);
-    if (!(d > 0.f)) return 0u;
-    const float inv = __fdiv_rn(1.f, d);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float lo = __uint_as_float((__float_as_uint(u[2 * i] * inv) + 0x20u) & ~0x3Fu);
-        const float hi = __uint_as_float((__float_as_uint(u[2 * i + 1] * inv) + 0x20u) & ~0x3Fu);
-        uint32_t b;
-        asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(b) : "f"(hi), "f"(lo));
-        if (i < 4) codes.x |= b << (8 * i);
-        else codes.y |= b << (8 * (i - 4));
+    for (int k = 0; k < 2; k++) {
+        uint32_t &c = k ? codes.y : codes.x;
+        const float *u = q + 8 * k;
+        asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+            "mov.b32 %0, {a, b, c, d};\n\t}"
+            : "=r"(c) : "f"(u[0]), "f"(u[1]), "f"(u[2]), "f"(u[3]), "f"(u[4]), "f"(u[5]), "f"(u[6]), "f"(u[7]));
     }
     return sb;
 }
@@ -141,9 +165,8 @@ __device__ __forceinline__ void put(const Args &a, int64_t row, int b, bool live
     if (a.atoms && first) *reinterpret_cast<uint32_t *>(a.atoms + atom_at(row, b >> 2, nks)) = v;
 }
 
-// One row per G threads. G = 32, a warp: no barrier between the row's maximum and its codes, and 16 wide loads of 128 B
-// in flight per lane (16384 x 4096 bf16: 66 us with a CTA per row). G = 256, a CTA, for rows that a warp cannot keep and
-// for so few rows that warps would leave SMs idle. Blocks past the KEEP a thread keeps are read again (from L2).
+// One row per G threads, 256 / G rows a CTA: few enough threads that each has several blocks' loads in flight, more for
+// few rows. Blocks past the KEEP a thread keeps are read again (from L2).
 template <typename T, int G>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a) {
     __shared__ uint32_t red[THREADS / 32];
@@ -151,25 +174,22 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a) {
     const int64_t row = blockIdx.x * (int64_t)(THREADS / G) + threadIdx.x / G;
     const bool in = row < a.M;   // a warp is all in or all out
     const T *x = static_cast<const T *>(a.x) + (in ? row : 0) * a.ldx;
-    Raw<T> keep[KEEP<T>];
+    Raw<T> keep[KEEP];
+    uint32_t top[KEEP];
     uint32_t m = 0;
     if (in) {
 #pragma unroll
-        for (int i = 0; i < KEEP<T>; i++)
+        for (int i = 0; i < KEEP; i++)
             if (t + i * G < a.nb) load16(x + (t + i * G) * 16, a.vec, keep[i]);
 #pragma unroll
-        for (int i = 0; i < KEEP<T>; i++)
-            if (t + i * G < a.nb) {
-                float f[16];
-                widen(keep[i], f);
-                m = max(m, amax_bits(f));
-            }
-        for (int b = t + KEEP<T> * G; b < a.nb; b += G) {
+        for (int i = 0; i < KEEP; i++) {
+            top[i] = t + i * G < a.nb ? block_max(keep[i]) : 0u;
+            m = max(m, top[i] & ~NONFINITE);
+        }
+        for (int b = t + KEEP * G; b < a.nb; b += G) {
             Raw<T> v;
-            float f[16];
             load16(x + (int64_t)b * 16, a.vec, v);
-            widen(v, f);
-            m = max(m, amax_bits(f));
+            m = max(m, block_max(v) & ~NONFINITE);
         }
     }
     m = __reduce_max_sync(0xffffffffu, m);
@@ -177,30 +197,29 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a) {
         if (!(threadIdx.x & 31)) red[threadIdx.x >> 5] = m;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < THREADS / 32; i++) m = max(m, red[i]);
+        for (int i = 0; i < G / 32; i++) m = max(m, red[threadIdx.x / G * (G / 32) + i]);
     }
     if (!in) return;
     const int e = scale_exp(m);
-    const float inv_s = pow2f(-e);
     if (t == 0) a.s[row] = pow2f(e);
     const int lim = (a.nb + 31) & ~31;   // whole warps, for the shuffles of put()
 #pragma unroll
-    for (int i = 0; i < KEEP<T>; i++) {
+    for (int i = 0; i < KEEP; i++) {
         const int b = t + i * G;
         if (b < lim) {
             uint2 c = make_uint2(0u, 0u);
             uint32_t sb = 0;
-            if (b < a.nb) sb = block16<T>(keep[i], inv_s, c);
+            if (b < a.nb) sb = block16<T>(keep[i], top[i], e, c);
             put(a, row, b, b < a.nb, c, sb);
         }
     }
-    for (int b = t + KEEP<T> * G; b < lim; b += G) {
+    for (int b = t + KEEP * G; b < lim; b += G) {
         uint2 c = make_uint2(0u, 0u);
         uint32_t sb = 0;
         if (b < a.nb) {
             Raw<T> v;
             load16(x + (int64_t)b * 16, a.vec, v);
-            sb = block16<T>(v, inv_s, c);
+            sb = block16<T>(v, block_max(v), e, c);
         }
         put(a, row, b, b < a.nb, c, sb);
     }
@@ -216,10 +235,8 @@ __global__ void __launch_bounds__(THREADS) tensor_scale_kernel(const Args a) {
         const T *x = static_cast<const T *>(a.x) + row * a.ldx;
         for (int b = blockIdx.x * THREADS + threadIdx.x; b < a.nb; b += gridDim.x * THREADS) {
             Raw<T> v;
-            float f[16];
             load16(x + (int64_t)b * 16, a.vec, v);
-            widen(v, f);
-            m = max(m, amax_bits(f));
+            m = max(m, block_max(v) & ~NONFINITE);
         }
     }
     m = __reduce_max_sync(0xffffffffu, m);
@@ -234,7 +251,7 @@ __global__ void __launch_bounds__(THREADS) tensor_scale_kernel(const Args a) {
 // Tensor scale, second pass.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) tensor_kernel(const Args a) {
-    const float inv_s = pow2f(127 - (int)(__float_as_uint(*a.s) >> 23));
+    const int e = (int)(__float_as_uint(*a.s) >> 23) - 127;
     const int lim = (a.nb + 31) & ~31;
     for (int64_t i = blockIdx.y; i < a.M; i += gridDim.y) {
         const int64_t row = a.M - 1 - i;   // the first pass ended with the last rows: L2 still holds those
@@ -245,7 +262,7 @@ __global__ void __launch_bounds__(THREADS) tensor_kernel(const Args a) {
             if (b < a.nb) {
                 Raw<T> v;
                 load16(x + (int64_t)b * 16, a.vec, v);
-                sb = block16<T>(v, inv_s, c);
+                sb = block16<T>(v, block_max(v), e, c);
             }
             put(a, row, b, b < a.nb, c, sb);
         }
@@ -255,12 +272,14 @@ __global__ void __launch_bounds__(THREADS) tensor_kernel(const Args a) {
 template <typename T>
 static int launch(const Args &a, bool per_row, cudaStream_t st, const DeviceInfo &di) {
     if (per_row) {
-        if (a.nb <= 32 || (a.nb <= 32 * KEEP<T> && a.M >= 8 * di.sms)) {
-            const int64_t g = (a.M + THREADS / 32 - 1) / (THREADS / 32);
-            rows_kernel<T, 32><<<(unsigned)g, THREADS, 0, st>>>(a);
-        } else {
-            rows_kernel<T, THREADS><<<(unsigned)a.M, THREADS, 0, st>>>(a);
-        }
+        // the fewest threads whose registers hold a row, or more while the rows leave room on the SMs
+        int g = 32;
+        while (g < THREADS && (a.nb > g * KEEP || (a.nb > g && a.M * g * 2 <= (int64_t)di.sms * 1024))) g *= 2;
+        const unsigned grid = (unsigned)((a.M + THREADS / g - 1) / (THREADS / g));
+        if (g == 32) rows_kernel<T, 32><<<grid, THREADS, 0, st>>>(a);
+        else if (g == 64) rows_kernel<T, 64><<<grid, THREADS, 0, st>>>(a);
+        else if (g == 128) rows_kernel<T, 128><<<grid, THREADS, 0, st>>>(a);
+        else rows_kernel<T, 256><<<grid, THREADS, 0, st>>>(a);
         return launch_status();
     }
     if (cudaMemsetAsync(a.s, 0, sizeof(float), st) != cudaSuccess) return QMOE_ERR_LAUNCH;

@@ -73,9 +73,10 @@ def dequant_rows(q, r0, r1, out):
         raise C.QmoeError("out must be contiguous")
     sc = q.get("sc")
     if q["fmt"] == "nvfp4_rows":
-        with _on(out):
-            C.call("dq_dequant_nvfp4", C.ptr(q["w"]), C.ptr(sc), C.ptr(q["s"]), 1, q["N"], q["K"], r0, r1, C.ptr(out),
-                   C.dtype_code(out), C.stream_of(out))
+        if r1 > r0:
+            with _on(out):
+                C.call("dq_dequant_nvfp4", C.ptr(q["w"]), C.ptr(sc), C.ptr(q["s"]), 1, q["N"], q["K"], r0, r1, C.ptr(out),
+                       C.dtype_code(out), C.stream_of(out))
         return out
     C.call("dq_dequant_rows", 0 if q["fmt"] == "fp8" else 1, C.ptr(q["w"]), C.ptr(sc) if sc is not None else None,
            C.ptr(q["s"]), q["N"], q["K"], r0, r1, C.ptr(out), C.dtype_code(out), C.stream_of(out))
@@ -158,8 +159,8 @@ def _atoms_bytes(rows, K):
     return (rows + 127) // 128 * ((K + 63) // 64) * 512
 
 
-def _no_grad(*ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+def _no_grad(t):
+    if t.requires_grad and torch.is_grad_enabled():
         raise C.QmoeError("the four-bit operators have no gradient: call them under torch.no_grad()")
 
 
@@ -174,11 +175,11 @@ def _rows(x):
     return x, dt, x.stride(0) if M > 1 else K
 
 
-def quantize(x, per_row=True):
+def quantize(x, per_row=True, for_gemm=False):
     """x [M, K] (bf16, fp16 or fp32; K a multiple of 16; rows may be strided) -> quantized dict: codes "w" [M, K/2],
     block scales "sc" [M, K/16] (e4m3 bytes), "s" f32 [M] with fmt "nvfp4_rows" (per_row), or [1] with fmt "nvfp4"
-    (one scale for the tensor: a weight of this module), and "sca", the scales as gemm reads them. s is the smallest
-    power of two with amax <= 2688 s, scales and codes the nearest, ties to even. A 16-element block that holds an
+    (one scale for the tensor: a weight of this module); with for_gemm also "sca", the scales as gemm reads them (what
+    prepare adds, in the same pass). s is the smallest power of two with amax <= 2688 s, scales and codes the nearest, ties to even. A 16-element block that holds an
     infinity or a NaN reads back as NaN; the others are as if that value were zero."""
     if x.dim() != 2:
         raise C.QmoeError("quantize takes a matrix [M, K]")
@@ -189,14 +190,18 @@ def quantize(x, per_row=True):
         raise C.QmoeError("a tensor without rows has no scale")
     x, dt, ld = _rows(x)
     dev = x.device
-    q = {"fmt": "nvfp4_rows" if per_row else "nvfp4", "w": torch.empty(M, K // 2, dtype=torch.uint8, device=dev),
-         "sc": torch.empty(M, K // 16, dtype=torch.uint8, device=dev),
-         "s": torch.empty(M if per_row else 1, dtype=torch.float32, device=dev), "N": M, "K": K,
-         "sca": torch.empty(_atoms_bytes(M, K), dtype=torch.uint8, device=dev)}
+    w = torch.empty(M, K // 2, dtype=torch.uint8, device=dev)
+    sc = torch.empty(M, K // 16, dtype=torch.uint8, device=dev)
+    s = torch.empty(M if per_row else 1, dtype=torch.float32, device=dev)
+    q = {"fmt": "nvfp4_rows" if per_row else "nvfp4", "w": w, "sc": sc, "s": s, "N": M, "K": K}
+    sca = None
+    if for_gemm:
+        q["sca"] = torch.empty(_atoms_bytes(M, K), dtype=torch.uint8, device=dev)
+        sca = q["sca"].data_ptr()
     if M:
         with _on(x):
-            C.call("dq_quantize_nvfp4", x.data_ptr(), dt, ld, M, K, int(per_row), q["w"].data_ptr(), q["sc"].data_ptr(),
-                   q["s"].data_ptr(), q["sca"].data_ptr(), C.stream_of(x))
+            C.call("dq_quantize_nvfp4", x.data_ptr(), dt, ld, M, K, int(per_row), w.data_ptr(), sc.data_ptr(), s.data_ptr(), sca,
+                   C.stream_of(x))
     return q
 
 
@@ -208,6 +213,8 @@ def prepare(q):
     if "sca" in q:
         return q
     N, K = q["N"], q["K"]
+    if N == 0:
+        return {**q, "sca": torch.empty(0, dtype=torch.uint8, device=q["sc"].device)}
     sc = q["sc"].contiguous()
     sca = torch.empty(_atoms_bytes(N, K), dtype=torch.uint8, device=sc.device)
     with _on(sc):
@@ -243,7 +250,7 @@ def _check_product(q, M, K, dtype, dev, act, residual):
 
 def gemm(q, xq, dtype=torch.bfloat16, act=None, residual=None):
     """y [M, N] in dtype = dequant(xq) @ dequant(q).T for two NVFP4 dicts (xq of quantize: activations; q: a weight,
-    best one that went through prepare, else its scales are laid out in this call), products exact, fp32 sums in a
+    either without "sca" has its scales laid out in this call), products exact, fp32 sums in a
     fixed order. act "relu2": relu(y)^2; residual [M, N] in dtype: y + residual; each on y rounded to dtype, as the
     unfused torch operators. K a multiple of 32."""
     if xq["fmt"] not in _NVFP4:

@@ -58,8 +58,11 @@ class _Route(torch.autograd.Function):
         return ids, w, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, _ids, dw, _counts):
+    def backward(ctx, *grads):
+        return (_Route.twice if torch.is_grad_enabled() else _Route.once)(ctx, *grads)
+
+    @staticmethod
+    def once(ctx, _ids, dw, _counts):
         if dw is None:
             return (None,) * 8
         logits, ids = ctx.saved_tensors
@@ -71,7 +74,9 @@ class _Route(torch.autograd.Function):
             with _on(x):
                 C.call("qmoe_route_backward", x.data_ptr(), C.DT[x.dtype], ld, x.shape[0], x.shape[1], top_k, norm, score, scaling,
                        ids.data_ptr(), C.ptr(dw), dl.data_ptr(), C.stream_of(x))
-        return (dl,) + (None,) * 7
+        return dl, None, None, None, None, None, None, None
+
+    twice = staticmethod(torch.autograd.function.once_differentiable(once.__func__))   # of a graph: refuses a second
 
 
 def route(logits, bias=None, top_k=22, scaling=5.0, n_group=1, topk_group=1, norm_topk_prob=False, score="sigmoid"):
@@ -131,8 +136,11 @@ class _Balance(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dloss, _counts):
+    def backward(ctx, *grads):
+        return (_Balance.twice if torch.is_grad_enabled() else _Balance.once)(ctx, *grads)
+
+    @staticmethod
+    def once(ctx, dloss, _counts):
         if dloss is None:
             return (None,) * 5
         logits, mask, c = ctx.saved_tensors
@@ -144,6 +152,8 @@ class _Balance(torch.autograd.Function):
                 C.call("qmoe_balance_backward", x.data_ptr(), C.DT[x.dtype], ld, mask.data_ptr() if mask is not None else None,
                        x.shape[0], x.shape[1], ctx.score, c.data_ptr(), C.ptr(g), dl.data_ptr(), C.stream_of(x))
         return dl, None, None, None, None
+
+    twice = staticmethod(torch.autograd.function.once_differentiable(once.__func__))
 
 
 def balance_loss(logits, ids, mask=None, score="sigmoid", coef=1.0):

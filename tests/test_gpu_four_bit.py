@@ -62,6 +62,9 @@ def check_quantized(q, x, per_row):
     assert torch.equal(q["s"].double(), s)
     assert torch.equal(torch.nan_to_num(scales_of(q), nan=-1.0), torch.nan_to_num(sc, nan=-1.0))
     assert torch.equal(codes_of(q), v)
+    if "sca" not in q:
+        import dense_q as D
+        q = D.prepare(q)
     # the same scales as atoms: row r of k-step ks at [r / 128][ks], (r % 32) * 16 + (r % 128 / 32) * 4
     M, nb = q["N"], q["K"] // 16
     nks = (nb + 3) // 4
@@ -80,7 +83,7 @@ def test_quantize(M, K, dtype, per_row):
     x = torch.randn(M, K, generator=g, device=DEV) * torch.exp(2 * torch.randn(M, 1, generator=g, device=DEV))
     x = x.to(dtype)
     x[M // 2, K // 2:K // 2 + 16] = 0
-    check_quantized(D.quantize(x, per_row), x, per_row)
+    check_quantized(D.quantize(x, per_row, True), x, per_row)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
@@ -135,18 +138,20 @@ def test_quantize_extremes(per_row):
     assert torch.isnan(back[6, 16:32]).all() and torch.isfinite(back[6, :16]).all() and torch.isfinite(back[6, 32:]).all()
     for dt in (torch.bfloat16, torch.float16):
         y = x[6:8].to(dt)
-        check_quantized(D.quantize(y, per_row), y, per_row)
+        check_quantized(D.quantize(y, per_row, True), y, per_row)
 
 
 def test_quantize_strides_and_offsets():
     import dense_q as D
     base = torch.randn(70, 1100, generator=seeded(9), device=DEV).to(torch.bfloat16)
     for x in (base[:, :1024], base[::3, 1:993], base[:, 8:1032], base.t()[:64].t()[:, :64], base[:1, :1088], base.t()[:1088, :64].t()):
-        check_quantized(D.quantize(x), x, True)
+        check_quantized(D.quantize(x, for_gemm=True), x, True)
         check_quantized(D.quantize(x, per_row=False), x, False)
     one = base[0, :16].reshape(1, 16).expand(5, 16)      # a broadcast row
     check_quantized(D.quantize(one), one, True)
-    assert D.quantize(base[:0, :64])["w"].shape == (0, 32)
+    empty = D.quantize(base[:0, :64])
+    assert empty["w"].shape == (0, 32) and D.dequant(empty).shape == (0, 64)
+    assert D.gemm(D.quantize(base[:4, :64]), empty).shape == (0, 4) and D.gemm(empty, D.quantize(base[:4, :64])).shape == (4, 0)
 
 
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
