@@ -63,12 +63,12 @@ __device__ __forceinline__ bool elect_one() {
     return v != 0;
 }
 
-// Bounded wait of a whole warp; the result is the same in every lane.
+// Bounded wait of a whole warp. The result comes from a vote, so that the compiler sees that it is the same in every lane.
 __device__ __forceinline__ bool all_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, long long limit) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     bool ok = true;
     if ((threadIdx.x & 31) == 0) ok = lane_wait(bar, parity, abort_flag, &g_status, limit);
-    ok = __shfl_sync(0xffffffffu, ok, 0);
+    ok = __all_sync(0xffffffffu, ok);
     if (ok) mbar_try_wait(bar, parity);   // a completed phase: the acquire of the other lanes
     return ok;
 }
@@ -340,10 +340,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 // Which operand has the 256 rows (the lanes of tensor memory) is the caller's choice: with the tokens there, a thread
 // holds consecutive columns of one row of y and stores 32 bytes at a time; with the weights there, a warp's lanes are
 // consecutive in a row of y, which suits rows of y that are not 32-byte aligned.
-// What is left is issue: a stage is 4 MMAs of 128 cycles and 12 scale copies, and one warp needs about 30 cycles for a
-// copy and 40 for an MMA. So one warp issues the copies, up to two stages ahead, and another the MMAs.
-constexpr int PAIR_THREADS = 224;   // warps 0..3 epilogue, 4 loads, 5 MMA, 6 scale copies
-
+// What is left is issue: a stage is 4 MMAs of 128 cycles, 12 scale copies, a wait and a commit, about 500 cycles of one
+// warp's time. They stand in one elected block per stage, the next stage's copies before this stage's MMAs, so that the
+// copies are done when their MMAs come up. (A warp of its own for the copies needs two more hand-offs per stage and
+// was slower: 192 us for 8192 x 12288 x 4096.)
 template <int TN> struct PairPlan {
     static constexpr int NA = (TN + 127) / 128;
     static constexpr int B_BYTES = TN / 2 * ROWB;
@@ -352,7 +352,7 @@ template <int TN> struct PairPlan {
     static constexpr int STAGE = (BYTES + 1023) / 1024 * 1024;
     static constexpr int STAGES = 221184 / STAGE < 8 ? 221184 / STAGE : 8;
     static constexpr int OFF_BAR = STAGES * STAGE;
-    static constexpr int NBAR = 2 * STAGES + 7;
+    static constexpr int NBAR = 2 * STAGES + 5;
     static constexpr int OFF_MISC = OFF_BAR + (NBAR * 8 + 15) / 16 * 16;
     static constexpr int SMEM = OFF_MISC + 16 + 1024;
     static_assert(SMEM <= 232448, "fits the 227 KB opt-in");
@@ -412,8 +412,33 @@ __device__ __forceinline__ uint32_t in_leader(const void *p) {   // the same pla
     return r;
 }
 
+// tmem_ld32 in two halves, so that several loads are in flight; the wait takes the registers, so that none is used before.
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+          "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+          "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+          "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_hold(float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i++) asm volatile("" : "+f"(v[i]));
+}
+__device__ __forceinline__ void tmem_ld_wait(float (&a)[32], float (&b)[32], float (&c)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    tmem_hold(a);
+    tmem_hold(b);
+    tmem_hold(c);
+}
+
+// Only tensor-memory reads come before it, and those are waited for. (With .release.cluster it waits for the thread's
+// global stores too: 1300 cycles.)
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -469,7 +494,7 @@ __device__ __forceinline__ void store_run(void *y, const void *res, int64_t at, 
 }
 
 template <int TN, typename T, int EPI>
-__global__ void __launch_bounds__(PAIR_THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 1)
     pair_kernel(const PairParams p, const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                 const __grid_constant__ CUtensorMap tm_sa, const __grid_constant__ CUtensorMap tm_sb) {
     using P = PairPlan<TN>;
@@ -482,8 +507,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     uint64_t *empty = full + S;
     uint64_t *acc_full = empty + S;      // [2]
     uint64_t *acc_free = acc_full + 2;   // [2], the first CTA's
-    uint64_t *sf_full = acc_free + 2;    // [2], the first CTA's: a slot's scales are in tensor memory
-    uint64_t *drain = sf_full + 2;
+    uint64_t *drain = acc_free + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + P::OFF_MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(sm + P::OFF_MISC + 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -498,9 +522,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         mbar_init(&acc_full[1], 1);
         mbar_init(&acc_free[0], 8);
         mbar_init(&acc_free[1], 8);
-        mbar_init(&sf_full[0], 1);
-        mbar_init(&sf_full[1], 1);
-        mbar_init(drain, 2);
+        mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -545,67 +567,50 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         }
         __syncwarp();
     } else if (warp == 5) {
-        // ------------------------------------------------------------ MMAs: the first CTA's warp drives both tensor cores
+        // ------------------------------------------------------------ the first CTA's warp drives both tensor cores
         if (rank == 0) {
             const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | (16u << 24);   // M = 256
-            uint32_t u = 0;
-            int s = 0, t = 0;
-            bool ok = true;
-            for (int i = first; i < p.ntiles && ok; i += step, t++) {
-                const uint32_t d = tmem + (t & 1) * P::ACC1;
-                const int f = t - P::LAG;
-                if (f >= 0 && !all_wait(&acc_free[f & 1], (f >> 1) & 1, abort_flag, p.wait)) break;
+            const bool lead = elect_one();
+            const uint32_t total = first < p.ntiles ? (uint32_t)((p.ntiles - first + step - 1) / step) * p.nst : 0u;
+            const int tail = p.nks - 4 * (p.nst - 1);   // k-steps of a tile's last stage
+            uint32_t ph = 0;                            // parity of stage s's current use
+            int s = 0, sp = 0, kt = 0, kp = 0, t = 0;   // sp, kp: of the stage before, whose MMAs are due
+            for (uint32_t u = 0; u <= total; u++) {
+                if (u < total && !all_wait(&full[s], ph, abort_flag, p.wait)) break;
+                if (u > 0 && kp == 0 && t >= P::LAG) {
+                    const int f = t - P::LAG;
+                    if (!all_wait(&acc_free[f & 1], (f >> 1) & 1, abort_flag, p.wait)) break;
+                }
                 tc_fence_after();
-                for (int kt = 0; kt < p.nst; kt++, u++) {
-                    if (!all_wait(&sf_full[u & 1], (u >> 1) & 1, abort_flag, p.wait)) {   // and so are the stage's codes
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t a = ((sbase + s * P::STAGE) >> 4) + LO, c = tmem + P::SF_COL + (u & 1) * P::SF_SLOT;
-                    const int nk = min(4, p.nks - 4 * kt);
-                    if (elect_one()) {
+                const uint32_t c = P::SF_COL + (u & 1) * P::SF_SLOT, cp = P::SF_COL + (~u & 1) * P::SF_SLOT;
+                const uint32_t f = ((sbase + s * P::STAGE + P::OFF_SFA) >> 4) + LO, a = ((sbase + sp * P::STAGE) >> 4) + LO;
+                const uint32_t d = (t & 1) * P::ACC1;
+                if (lead) {
+                    if (u < total) {
+                        const int nk = kt == p.nst - 1 ? tail : 4;
 #pragma unroll
                         for (int kk = 0; kk < 4; kk++) {
                             if (kk >= nk) break;
-                            mma_pair(d, a + 2 * kk, a + (P::OFF_B >> 4) + 2 * kk, idesc, (kt > 0) | (kk > 0), c + kk * 4 * (1 + P::NA), c + kk * 4 * (1 + P::NA) + 4);
+                            cp_sf_pair(c + kk * 4 * (1 + P::NA), f + kk * (ATOM >> 4));
+#pragma unroll
+                            for (int a = 0; a < P::NA; a++)
+                                cp_sf_pair(c + kk * 4 * (1 + P::NA) + 4 + 4 * a, f + ((SFA_BYTES + a * SFA_BYTES + kk * ATOM) >> 4));
                         }
-                        commit_pair(&empty[s]);
-                        if (kt == p.nst - 1) commit_pair(&acc_full[t & 1]);
                     }
-                    __syncwarp();
-                    s = s + 1 == S ? 0 : s + 1;
-                }
-            }
-        }
-        __syncwarp();
-    } else if (warp == 6) {
-        // ------------------------------------------------------------ scales to tensor memory, for both CTAs
-        if (rank == 0) {
-            const uint32_t total = (uint32_t)((p.ntiles - first + step - 1) / step) * p.nst;
-            uint32_t ph = 0, last = 0;   // parity of stage s's current use, and of the use two stages before
-            int s = 0, s2 = 0, kt = 0;
-            for (uint32_t u = 0; u < total; u++) {
-                if (!all_wait(&full[s], ph, abort_flag, p.wait)) break;
-                if (u >= 2) {   // the slot's last MMAs have completed
-                    if (!all_wait(&empty[s2], last, abort_flag, p.wait)) break;
-                    if (++s2 == S) s2 = 0, last ^= 1;
-                }
-                tc_fence_after();
-                const uint32_t f = ((sbase + s * P::STAGE + P::OFF_SFA) >> 4) + LO, c = tmem + P::SF_COL + (u & 1) * P::SF_SLOT;
-                const int nk = min(4, p.nks - 4 * kt);
-                if (elect_one()) {
+                    if (u > 0) {
+                        const int nk = kp == p.nst - 1 ? tail : 4;
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++) {
-                        if (kk >= nk) break;
-                        cp_sf_pair(c + kk * 4 * (1 + P::NA), f + kk * (ATOM >> 4));
-#pragma unroll
-                        for (int a = 0; a < P::NA; a++)
-                            cp_sf_pair(c + kk * 4 * (1 + P::NA) + 4 + 4 * a, f + ((SFA_BYTES + a * SFA_BYTES + kk * ATOM) >> 4));
+                        for (int kk = 0; kk < 4; kk++) {
+                            if (kk >= nk) break;
+                            mma_pair(d, a + 2 * kk, a + (P::OFF_B >> 4) + 2 * kk, idesc, kp + kk, cp + kk * 4 * (1 + P::NA), cp + kk * 4 * (1 + P::NA) + 4);
+                        }
+                        commit_pair(&empty[sp]);
+                        if (kp == p.nst - 1) commit_pair(&acc_full[t & 1]);
                     }
-                    commit_one(&sf_full[u & 1]);
                 }
                 __syncwarp();
+                if (u > 0 && kp == p.nst - 1) t++;
+                sp = s, kp = kt;
                 if (++s == S) s = 0, ph ^= 1;
                 if (++kt == p.nst) kt = 0;
             }
@@ -615,11 +620,12 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         // ------------------------------------------------------------ epilogue: each CTA its 128 lanes
         int t = 0;
         for (int i = first; i < p.ntiles; i += step, t++) {
-            if (!all_wait(&acc_full[t & 1], (t >> 1) & 1, abort_flag, p.wait)) break;
-            tc_fence_after();
             const int a = i % p.nba * 256 + rank * 128 + tid, b0 = i / p.nba * TN;
             const uint32_t d = tmem + (t & 1) * P::ACC1 + ((uint32_t)(warp * 32) << 16);
             const float sa = a < p.A ? p.sa[(int64_t)a * p.sa_step] : 0.f;
+            const uint32_t free_bar = in_leader(&acc_free[t & 1]);
+            if (!all_wait(&acc_full[t & 1], (t >> 1) & 1, abort_flag, p.wait)) break;
+            tc_fence_after();
             const bool in = a < p.A;
             auto put = [&](int c0, const float(&v)[32]) {
                 const int left = p.B - b0 - c0;   // columns from here that exist
@@ -637,15 +643,16 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
             auto release = [&] {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_remote(in_leader(&acc_free[t & 1]));
+                if (lane == 0) arrive_remote(free_bar);
             };
             if constexpr (TN == 256) {
                 // the 96 columns shared with the other accumulator first (accumulator 0's last, 1's first)
                 const int c0 = t & 1 ? 0 : 160, c1 = t & 1 ? 96 : 0;
                 float v0[32], v1[32], v2[32];
-                tmem_ld32(d + c0, v0);
-                tmem_ld32(d + c0 + 32, v1);
-                tmem_ld32(d + c0 + 64, v2);
+                tmem_ld32_issue(d + c0, v0);
+                tmem_ld32_issue(d + c0 + 32, v1);
+                tmem_ld32_issue(d + c0 + 64, v2);
+                tmem_ld_wait(v0, v1, v2);
                 release();
                 put(c0, v0);
                 put(c0 + 32, v1);
@@ -674,7 +681,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         if (warp == 4 && rank == 0)
             for (uint32_t u = q > (uint32_t)S ? q - S : 0; u < q; u++) mbar_wait(&full[u % S], (u / S) & 1);
     }
-    if ((warp == 5 || warp == 6) && rank == 0 && *abort_flag) {   // the lane that issued: elect picks the same one
+    if (warp == 5 && rank == 0 && *abort_flag) {   // the lane that issued: elect picks the same one
         if (elect_one()) {
             commit_one(drain);
             mbar_wait(drain, 0);
@@ -775,7 +782,7 @@ static int launch_pair(const Params &g, const uint8_t *w, const uint8_t *x, int6
     cudaLaunchConfig_t cfg = {};
     const int pairs = di.sms / 2;
     cfg.gridDim = dim3((unsigned)(2 * (p.ntiles < pairs ? p.ntiles : pairs)));
-    cfg.blockDim = dim3(PAIR_THREADS);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = PairPlan<TN>::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
