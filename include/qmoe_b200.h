@@ -328,12 +328,15 @@ int dq_gemm_nvfp4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int
                   const uint8_t *x_atoms, const float *sx, int sx_per_row, int M, int N, int K, int epilogue,
                   const void *residual, void *y, int y_dtype, void *stream);
 
-/* dq_quantize_nvfp4 (per row) and dq_gemm_nvfp4 in one call: y [M, N] in x_dtype from x [M, K], rows ldx elements apart.
- * The workspace (16-byte aligned; dq_linear_a4_workspace_bytes(M, K), 0 for sizes out of range) holds the quantized
- * rows and needs no initial value; it must not be used by another call running concurrently. */
+/* dq_quantize_nvfp4 (per row) and dq_gemm_nvfp4 in one call: y [M, N] in x_dtype from x [M, K], rows ldx elements apart,
+ * and a weight given with its scales both as stored (w_sc [N, K/16]) and as atoms. Up to four rows run as one kernel that
+ * quantizes and multiplies (the sums then run in another order). The workspace (16-byte aligned;
+ * dq_linear_a4_workspace_bytes(M, K), 0 for sizes out of range; not looked at, so possibly NULL, for M <= 4 with
+ * K <= 16384) holds the quantized rows and needs no initial value; it must not be used by another call running
+ * concurrently. */
 size_t dq_linear_a4_workspace_bytes(int64_t M, int64_t K);
-int dq_linear_a4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int sw_per_row, const void *x, int x_dtype,
-                 int64_t ldx, int M, int N, int K, int epilogue, const void *residual, void *y, void *workspace,
+int dq_linear_a4(const uint8_t *w, const uint8_t *w_sc, const uint8_t *w_atoms, const float *sw, int sw_per_row, const void *x,
+                 int x_dtype, int64_t ldx, int M, int N, int K, int epilogue, const void *residual, void *y, void *workspace,
                  size_t workspace_bytes, void *stream);
 
 /* The first error the calls of dq_gemm_nvfp4 on the current device recorded since the last clear; waits for stream. */

@@ -60,7 +60,7 @@ SIGNATURES = {
     "dq_dequant_nvfp4": (_i, [_p, _p, _p, _i, _i64, _i64, _i64, _i64, _p, _i, _p]),
     "dq_gemm_nvfp4": (_i, [_p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i, _p]),
     "dq_linear_a4_workspace_bytes": (_sz, [_i64, _i64]),
-    "dq_linear_a4": (_i, [_p, _p, _p, _i, _p, _i, _i64, _i, _i, _i, _i, _p, _p, _p, _sz, _p]),
+    "dq_linear_a4": (_i, [_p, _p, _p, _p, _i, _p, _i, _i64, _i, _i, _i, _i, _p, _p, _p, _sz, _p]),
     "dq_gemm_nvfp4_status": (_i, [_i, _p]),
     "dq_dequant_rows": (_i, [_i, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _i, _p]),
 }

@@ -8,6 +8,7 @@
 // k-step). One thread copies the stage's atoms to tensor memory (tcgen05.cp) and issues its MMAs; the tensor pipe runs
 // both in the order issued, so the scale slots, two of them, need no barrier.
 #include "common.cuh"
+#include "epilogue4.cuh"
 #include "host.h"
 #include "tc.cuh"
 
@@ -89,37 +90,11 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
-                 : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr, int rank) {
+    float4 v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
     return v;
-}
-
-// Results. The linear's value is rounded to the output type, then (in fp32, rounded again) its squared ReLU or the sum
-// with the residual, as the unfused operators round (no fused multiply-add). EPI is a template argument and its switch
-// stands outside the unrolled columns: with it inside, the epilogue's code no longer fitted the instruction cache and
-// 32 columns took 2,400 cycles instead of 200.
-template <typename T> __device__ __forceinline__ T narrow(float v);
-template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
-__device__ __forceinline__ float wide(float v) { return v; }
-__device__ __forceinline__ float wide(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float wide(__half v) { return __half2float(v); }
-
-// sx * sw * v and its epilogue, before the last rounding.
-template <typename T, int EPI> __device__ __forceinline__ float finish(float v, float sx, float sw, float res) {
-    v = __fmul_rn(__fmul_rn(v, sx), sw);
-    if (EPI == 1) {
-        const float o = wide(narrow<T>(v)), r = o > 0.f ? o : (o != o ? o : 0.f);
-        return __fmul_rn(r, r);
-    }
-    return EPI == 2 ? __fadd_rn(wide(narrow<T>(v)), res) : v;
-}
-
-template <typename T, int EPI> __device__ __forceinline__ void store_one(void *y, const void *res, int64_t at, float v, float sx, float sw) {
-    static_cast<T *>(y)[at] = narrow<T>(finish<T, EPI>(v, sx, sw, EPI == 2 ? wide(static_cast<const T *>(res)[at]) : 0.f));
 }
 
 // 32 tokens' columns of one weight row (a lane): element j at y[at + j * N], for the first `left` of them. Lane j of the
@@ -179,6 +154,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    pdl_wait();   // what comes before may write an operand: nothing of it is read earlier
     uint32_t q = 0;   // stages loaded (warp 4) or consumed (warp 5)
 
     if (warp == 4) {
@@ -298,16 +274,26 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncthreads();
         cluster_sync();
         const int n0 = first % p.nbn * BM, m0 = first / p.nbn * TN, total = min(TN, p.M - m0) * BM;
-        for (int e = part * THREADS + tid; e < total; e += split * THREADS) {
-            float v = 0.f;
-            for (int r = 0; r < split; r++) v += ld_cluster(sbase + e * 4, r);
+        for (int e = (part * THREADS + tid) * 4; e < total; e += split * THREADS * 4) {   // four weight rows of a token
+            float4 v[MAX_SPLIT];
+#pragma unroll
+            for (int r = 0; r < MAX_SPLIT; r++)
+                if (r < split) v[r] = ld_cluster(sbase + e * 4, r);   // all in flight together
+            float4 o = v[0];
+#pragma unroll
+            for (int r = 1; r < MAX_SPLIT; r++)
+                if (r < split) o.x += v[r].x, o.y += v[r].y, o.z += v[r].z, o.w += v[r].w;
             const int n = n0 + e % BM, m = m0 + e / BM;
-            if (n < p.N) {
-                const float sx = p.sx[(int64_t)m * p.sx_step], sw = p.sw[(int64_t)n * p.sw_step];
-                const int64_t at = (int64_t)m * p.N + n;
-                if (p.epilogue == 0) store_one<T, 0>(p.y, p.res, at, v, sx, sw);
-                else if (p.epilogue == 1) store_one<T, 1>(p.y, p.res, at, v, sx, sw);
-                else store_one<T, 2>(p.y, p.res, at, v, sx, sw);
+            const float sx = p.sx[(int64_t)m * p.sx_step];
+            const int64_t at = (int64_t)m * p.N + n;
+            const float u[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (n + j >= p.N) break;
+                const float sw = p.sw[(int64_t)(n + j) * p.sw_step];
+                if (p.epilogue == 0) store_one<T, 0>(p.y, p.res, at + j, u[j], sx, sw);
+                else if (p.epilogue == 1) store_one<T, 1>(p.y, p.res, at + j, u[j], sx, sw);
+                else store_one<T, 2>(p.y, p.res, at + j, u[j], sx, sw);
             }
         }
         cluster_sync();   // no CTA leaves while another reads its sums
@@ -340,10 +326,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 // Which operand has the 256 rows (the lanes of tensor memory) is the caller's choice: with the tokens there, a thread
 // holds consecutive columns of one row of y and stores 32 bytes at a time; with the weights there, a warp's lanes are
 // consecutive in a row of y, which suits rows of y that are not 32-byte aligned.
-// What is left is issue: a stage is 4 MMAs of 128 cycles, 12 scale copies, a wait and a commit, about 500 cycles of one
-// warp's time. They stand in one elected block per stage, the next stage's copies before this stage's MMAs, so that the
-// copies are done when their MMAs come up. (A warp of its own for the copies needs two more hand-offs per stage and
-// was slower: 192 us for 8192 x 12288 x 4096.)
+// One warp issues everything for both tensor cores, a stage in one elected block: the scale copies of k-step k + 1, then
+// the MMA of k-step k, so that a copy runs while the MMA before it does. The pipe runs them in the order issued, which
+// makes two k-steps' worth of scale columns enough. (Two stages' worth, with a warp of its own for the copies, needed two
+// more hand-offs per stage.) Without any loads the same work takes 0.96 of the time: what bounds it is the tensor pipe,
+// about 570 cycles of MMAs and 160 of copies a stage, at the clock the power limit leaves.
 template <int TN> struct PairPlan {
     static constexpr int NA = (TN + 127) / 128;
     static constexpr int B_BYTES = TN / 2 * ROWB;
@@ -354,11 +341,14 @@ template <int TN> struct PairPlan {
     static constexpr int OFF_BAR = STAGES * STAGE;
     static constexpr int NBAR = 2 * STAGES + 5;
     static constexpr int OFF_MISC = OFF_BAR + (NBAR * 8 + 15) / 16 * 16;
-    static constexpr int SMEM = OFF_MISC + 16 + 1024;
+    static constexpr int OFF_COL = OFF_MISC + 16;   // [4][TN] each epilogue warp's copy of the columns' scales of its tile
+    static constexpr int SMEM = OFF_COL + 4 * TN * 4 + 1024;
     static_assert(SMEM <= 232448, "fits the 227 KB opt-in");
-    static constexpr int ACC1 = TN == 256 ? 160 : TN;   // as Plan: at TN = 256 the accumulators share 96 columns
+    // Tensor memory: two accumulators and two k-steps of scales. At TN = 256 the accumulators share 32 columns, which the
+    // epilogue reads first, so that the next tile's MMAs wait for those alone; else for the tile before the last.
+    static constexpr int ACC1 = TN == 256 ? 224 : TN;
     static constexpr int SF_COL = ACC1 + TN;
-    static constexpr int SF_SLOT = 4 * 4 * (1 + NA);
+    static constexpr int SF_SLOT = 4 * (1 + NA);
     static constexpr int LAG = TN == 256 ? 1 : 2;
     static_assert(SF_COL + 2 * SF_SLOT <= 512, "tensor memory");
 };
@@ -424,15 +414,10 @@ __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, float (&v)[32]) 
           "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_hold(float (&v)[32]) {
+__device__ __forceinline__ void tmem_ld_wait(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; i++) asm volatile("" : "+f"(v[i]));
-}
-__device__ __forceinline__ void tmem_ld_wait(float (&a)[32], float (&b)[32], float (&c)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    tmem_hold(a);
-    tmem_hold(b);
-    tmem_hold(c);
 }
 
 // Only tensor-memory reads come before it, and those are waited for. (With .release.cluster it waits for the thread's
@@ -467,9 +452,9 @@ __device__ __forceinline__ void ld32(const void *p, uint32_t (&v)[8]) {
 }
 
 // 32 weight rows' columns of one token (a lane): y[at ..], for the first `left` of them, 32 bytes at a time (left, like the
-// row length, is a multiple of those). sw: one for all, or lane j's register holds column j's.
-template <typename T, int EPI>
-__device__ __forceinline__ void store_run(void *y, const void *res, int64_t at, bool in, int left, const float (&v)[32], float sx, float sw, bool each) {
+// row length, is a multiple of those). EACH: cs holds the columns' scales, else sw is all of theirs.
+template <typename T, int EPI, bool EACH>
+__device__ __forceinline__ void store_run(void *y, const void *res, int64_t at, bool in, int left, const float (&v)[32], float sx, float sw, const float *cs) {
     constexpr int EPV = 32 / sizeof(T);   // elements per store
 #pragma unroll
     for (int u = 0; u < 32 / EPV; u++) {
@@ -480,17 +465,26 @@ __device__ __forceinline__ void store_run(void *y, const void *res, int64_t at, 
         for (int j = 0; j < 8; j++) {
             if constexpr (sizeof(T) == 4) {
                 const int c = u * EPV + j;
-                o[j] = __float_as_uint(finish<T, EPI>(v[c], sx, each ? __shfl_sync(0xffffffffu, sw, c) : sw, __uint_as_float(r[j])));
+                o[j] = __float_as_uint(finish<T, EPI>(v[c], sx, EACH ? cs[c] : sw, __uint_as_float(r[j])));
             } else {
                 const int c = u * EPV + 2 * j;
                 const float2 q = unpack2(r[j], T{});
-                const float lo = finish<T, EPI>(v[c], sx, each ? __shfl_sync(0xffffffffu, sw, c) : sw, q.x);
-                const float hi = finish<T, EPI>(v[c + 1], sx, each ? __shfl_sync(0xffffffffu, sw, c + 1) : sw, q.y);
+                const float lo = finish<T, EPI>(v[c], sx, EACH ? cs[c] : sw, q.x);
+                const float hi = finish<T, EPI>(v[c + 1], sx, EACH ? cs[c + 1] : sw, q.y);
                 o[j] = pack2<T>(lo, hi);
             }
         }
         if (live) st32(static_cast<T *>(y) + at + u * EPV, o);
     }
+}
+
+// 32 tokens' columns of one weight row (a lane), their scales in cs.
+template <typename T, int EPI>
+__device__ __forceinline__ void store_tokens(void *y, const void *res, int64_t at, int64_t N, bool in, int left, const float (&v)[32], float sw, const float *cs) {
+    if (!in) return;
+#pragma unroll
+    for (int j = 0; j < 32; j++)
+        if (j < left) store_one<T, EPI>(y, res, at + j * N, v[j], cs[j], sw);
 }
 
 template <int TN, typename T, int EPI>
@@ -533,9 +527,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_before();
     __syncthreads();
     cluster_sync();   // both CTAs' barriers exist before either is signalled
-    tc_fence_after();
-    constexpr uint32_t tmem = 0;   // all 512 columns are this CTA's: they start at column 0
-    uint32_t q = 0;                // stages loaded
+    tc_fence_after();   // all 512 columns are this CTA's, so they start at column 0
+    pdl_wait();         // what comes before may write an operand: nothing of it is read earlier
+    uint32_t q = 0;     // stages loaded
 
     if (warp == 4) {
         // ------------------------------------------------------------ loads: each CTA its own half of the stage
@@ -571,105 +565,116 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (rank == 0) {
             const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | (16u << 24);   // M = 256
             const bool lead = elect_one();
-            const uint32_t total = first < p.ntiles ? (uint32_t)((p.ntiles - first + step - 1) / step) * p.nst : 0u;
             const int tail = p.nks - 4 * (p.nst - 1);   // k-steps of a tile's last stage
             uint32_t ph = 0;                            // parity of stage s's current use
-            int s = 0, sp = 0, kt = 0, kp = 0, t = 0;   // sp, kp: of the stage before, whose MMAs are due
-            for (uint32_t u = 0; u <= total; u++) {
-                if (u < total && !all_wait(&full[s], ph, abort_flag, p.wait)) break;
-                if (u > 0 && kp == 0 && t >= P::LAG) {
-                    const int f = t - P::LAG;
-                    if (!all_wait(&acc_free[f & 1], (f >> 1) & 1, abort_flag, p.wait)) break;
-                }
-                tc_fence_after();
-                const uint32_t c = P::SF_COL + (u & 1) * P::SF_SLOT, cp = P::SF_COL + (~u & 1) * P::SF_SLOT;
-                const uint32_t f = ((sbase + s * P::STAGE + P::OFF_SFA) >> 4) + LO, a = ((sbase + sp * P::STAGE) >> 4) + LO;
+            int s = 0, sp = 0, t = 0;                   // sp: the stage before
+            bool ok = true;
+            for (int i = first; i < p.ntiles && ok; i += step, t++) {
                 const uint32_t d = (t & 1) * P::ACC1;
-                if (lead) {
-                    if (u < total) {
-                        const int nk = kt == p.nst - 1 ? tail : 4;
-#pragma unroll
-                        for (int kk = 0; kk < 4; kk++) {
-                            if (kk >= nk) break;
-                            cp_sf_pair(c + kk * 4 * (1 + P::NA), f + kk * (ATOM >> 4));
-#pragma unroll
-                            for (int a = 0; a < P::NA; a++)
-                                cp_sf_pair(c + kk * 4 * (1 + P::NA) + 4 + 4 * a, f + ((SFA_BYTES + a * SFA_BYTES + kk * ATOM) >> 4));
+                const uint32_t off = (uint32_t)(i / p.nba * TN & 127) >> 5;   // TN = 192: a tile may start at row 64 of an atom
+                for (int kt = 0; kt < p.nst; kt++) {
+                    if (!all_wait(&full[s], ph, abort_flag, p.wait)) {
+                        ok = false;
+                        break;
+                    }
+                    if (kt == 0 && t >= P::LAG) {
+                        const int f = t - P::LAG;
+                        if (!all_wait(&acc_free[f & 1], (f >> 1) & 1, abort_flag, p.wait)) {
+                            ok = false;
+                            break;
                         }
                     }
-                    if (u > 0) {
-                        const int nk = kp == p.nst - 1 ? tail : 4;
+                    tc_fence_after();
+                    const uint32_t f = ((sbase + s * P::STAGE + P::OFF_SFA) >> 4) + LO;
+                    const uint32_t a = ((sbase + s * P::STAGE) >> 4) + LO, ap = ((sbase + sp * P::STAGE) >> 4) + LO;
+                    const int nk = kt == p.nst - 1 ? tail : 4;
+                    auto copies = [&](int k) {
+                        const uint32_t c = P::SF_COL + (k & 1) * P::SF_SLOT;
+                        cp_sf_pair(c, f + k * (ATOM >> 4));
 #pragma unroll
-                        for (int kk = 0; kk < 4; kk++) {
-                            if (kk >= nk) break;
-                            mma_pair(d, a + 2 * kk, a + (P::OFF_B >> 4) + 2 * kk, idesc, kp + kk, cp + kk * 4 * (1 + P::NA), cp + kk * 4 * (1 + P::NA) + 4);
+                        for (int j = 0; j < P::NA; j++) cp_sf_pair(c + 4 + 4 * j, f + ((SFA_BYTES + j * SFA_BYTES + k * ATOM) >> 4));
+                    };
+                    auto mma = [&](uint32_t at, int k, uint32_t acc) {
+                        const uint32_t c = P::SF_COL + (k & 1) * P::SF_SLOT;
+                        mma_pair(d, at + 2 * k, at + (P::OFF_B >> 4) + 2 * k, idesc, acc, c, c + 4 + off);
+                    };
+                    if (lead) {
+                        copies(0);
+                        if (kt > 0) {   // the stage before had four
+                            mma(ap, 3, 1);
+                            commit_pair(&empty[sp]);
                         }
-                        commit_pair(&empty[sp]);
-                        if (kp == p.nst - 1) commit_pair(&acc_full[t & 1]);
+#pragma unroll
+                        for (int k = 1; k < 4; k++)
+                            if (k < nk) {
+                                copies(k);
+                                mma(a, k - 1, kt + k - 1);
+                            }
+                        if (kt == p.nst - 1) {
+                            mma(a, nk - 1, kt + nk - 1);
+                            commit_pair(&empty[s]);
+                            commit_pair(&acc_full[t & 1]);
+                        }
                     }
+                    __syncwarp();
+                    sp = s;
+                    if (++s == S) s = 0, ph ^= 1;
                 }
-                __syncwarp();
-                if (u > 0 && kp == p.nst - 1) t++;
-                sp = s, kp = kt;
-                if (++s == S) s = 0, ph ^= 1;
-                if (++kt == p.nst) kt = 0;
             }
         }
         __syncwarp();
     } else {
         // ------------------------------------------------------------ epilogue: each CTA its 128 lanes
+        const bool each = p.sb_step != 0;
+        const float sb_all = p.sb[0];
+        float *cs = reinterpret_cast<float *>(sm + P::OFF_COL) + warp * TN;   // a copy per warp: no barrier between warps
         int t = 0;
         for (int i = first; i < p.ntiles; i += step, t++) {
             const int a = i % p.nba * 256 + rank * 128 + tid, b0 = i / p.nba * TN;
-            const uint32_t d = tmem + (t & 1) * P::ACC1 + ((uint32_t)(warp * 32) << 16);
-            const float sa = a < p.A ? p.sa[(int64_t)a * p.sa_step] : 0.f;
+            const uint32_t d = (t & 1) * P::ACC1 + ((uint32_t)(warp * 32) << 16);
+            const bool in = a < p.A;
+            const float sa = in ? p.sa[(int64_t)a * p.sa_step] : 0.f;
+            __syncwarp();
+            if (each || !p.tokens_on_lanes)
+#pragma unroll
+                for (int c = lane; c < TN; c += 32) cs[c] = b0 + c < p.B ? p.sb[(int64_t)(b0 + c) * p.sb_step] : 0.f;
+            __syncwarp();
             const uint32_t free_bar = in_leader(&acc_free[t & 1]);
             if (!all_wait(&acc_full[t & 1], (t >> 1) & 1, abort_flag, p.wait)) break;
             tc_fence_after();
-            const bool in = a < p.A;
             auto put = [&](int c0, const float(&v)[32]) {
                 const int left = p.B - b0 - c0;   // columns from here that exist
                 if (left <= 0) return;
-                const bool each = p.sb_step != 0;
-                const float sb = p.sb[each ? b0 + c0 + min(lane, left - 1) : 0];
-                if (p.tokens_on_lanes) {
-                    const int64_t at = (int64_t)a * p.N + b0 + c0;
-                    if (each) store_run<T, EPI>(p.y, p.res, at, in, left, v, sa, sb, true);
-                    else store_run<T, EPI>(p.y, p.res, at, in, left, v, sa, sb, false);
+                if (!p.tokens_on_lanes) {
+                    store_tokens<T, EPI>(p.y, p.res, (int64_t)(b0 + c0) * p.N + a, p.N, in, left, v, sa, cs + c0);
                 } else {
-                    store_columns<T, EPI>(p.y, p.res, (int64_t)(b0 + c0) * p.N + a, p.N, in, left, v, sb, sa);
+                    const int64_t at = (int64_t)a * p.N + b0 + c0;
+                    if (each) store_run<T, EPI, true>(p.y, p.res, at, in, left, v, sa, 0.f, cs + c0);
+                    else store_run<T, EPI, false>(p.y, p.res, at, in, left, v, sa, sb_all, cs);
                 }
             };
+            // the 32 columns shared with the other accumulator first (accumulator 0's last, 1's first); a run is loaded while
+            // the one before it is stored
+            const int start = TN == 256 && !(t & 1) ? 224 : 0;
+            auto at = [&](int k) { const int c = start + 32 * k; return c >= TN ? c - TN : c; };
+            float v0[32], v1[32];
+            tmem_ld32_issue(d + at(0), v0);
+            tmem_ld_wait(v0);
             auto release = [&] {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) arrive_remote(free_bar);
             };
-            if constexpr (TN == 256) {
-                // the 96 columns shared with the other accumulator first (accumulator 0's last, 1's first)
-                const int c0 = t & 1 ? 0 : 160, c1 = t & 1 ? 96 : 0;
-                float v0[32], v1[32], v2[32];
-                tmem_ld32_issue(d + c0, v0);
-                tmem_ld32_issue(d + c0 + 32, v1);
-                tmem_ld32_issue(d + c0 + 64, v2);
-                tmem_ld_wait(v0, v1, v2);
-                release();
-                put(c0, v0);
-                put(c0 + 32, v1);
-                put(c0 + 64, v2);
+            if (TN == 256) release();
 #pragma unroll 1
-                for (int u = 0; u < 160; u += 32) {
-                    tmem_ld32(d + c1 + u, v0);
-                    put(c1 + u, v0);
-                }
-            } else {
-#pragma unroll 1
-                for (int u = 0; u < TN; u += 32) {
-                    float v[32];
-                    tmem_ld32(d + u, v);
-                    if (u == TN - 32) release();
-                    put(u, v);
-                }
+            for (int k = 0; k < TN / 32; k += 2) {
+                tmem_ld32_issue(d + at(k + 1), v1);
+                put(at(k), v0);
+                tmem_ld_wait(v1);
+                if (k + 2 < TN / 32) tmem_ld32_issue(d + at(k + 2), v0);
+                else if (TN < 256) release();
+                put(at(k + 1), v1);
+                if (k + 2 < TN / 32) tmem_ld_wait(v0);
             }
         }
     }
@@ -691,7 +696,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     cluster_sync();   // neither CTA leaves while the other may still signal it or run on its memory
     if (warp == 5) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(*tmem_slot) : "memory");
     }
 }
 
@@ -716,7 +721,7 @@ static int launch(Params p, const CUtensorMap &a, const uint8_t *x, int64_t byte
     if (!(done.load(std::memory_order_acquire) >> (dev & 63) & 1) && !ensure_smem(kern, P::SMEM, dev, done)) return QMOE_ERR_LAUNCH;
     p.ntiles = p.nbn * ((p.M + TN - 1) / TN);
     p.split = 1;
-    if constexpr (TN <= 128) {   // too few tiles for the SMs: a cluster per tile, each CTA an even part of the stages
+    {   // too few tiles for the SMs: a cluster per tile, each CTA an even part of the stages
         int s = di.sms / p.ntiles;
         s = s < 1 ? 1 : s > MAX_SPLIT ? MAX_SPLIT : s;
         if (s > p.nst) s = p.nst;
@@ -728,12 +733,14 @@ static int launch(Params p, const CUtensorMap &a, const uint8_t *x, int64_t byte
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = P::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)p.split;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, kern, p, a, b) != cudaSuccess) {
         cudaGetLastError();
         return QMOE_ERR_LAUNCH;
@@ -752,13 +759,17 @@ static bool atom_map(CUtensorMap *m, const void *base, int64_t rows, int nks) {
               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Tokens on the lanes wherever y's rows allow 32-byte stores.
+template <typename T> static bool tokens_on_lanes(const Params &g) {
+    return (int64_t)g.N * sizeof(T) % 32 == 0 && !((reinterpret_cast<uintptr_t>(g.y) | reinterpret_cast<uintptr_t>(g.res)) & 31u);
+}
+
 template <int TN, typename T, int EPI>
 static int launch_pair(const Params &g, const uint8_t *w, const uint8_t *x, int64_t bytes, cudaStream_t st, int dev, const DeviceInfo &di) {
     static std::atomic<uint64_t> done{0};
     auto kern = pair_kernel<TN, T, EPI>;
     PairParams p{};
-    // tokens on the lanes wherever y's rows allow 32-byte stores
-    p.tokens_on_lanes = (int64_t)g.N * sizeof(T) % 32 == 0 && !((reinterpret_cast<uintptr_t>(g.y) | reinterpret_cast<uintptr_t>(g.res)) & 31u);
+    p.tokens_on_lanes = tokens_on_lanes<T>(g);
     const bool t = p.tokens_on_lanes;
     p.sa = t ? g.sx : g.sw;
     p.sb = t ? g.sw : g.sx;
@@ -785,12 +796,14 @@ static int launch_pair(const Params &g, const uint8_t *w, const uint8_t *x, int6
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = PairPlan<TN>::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, kern, p, a, b, sa, sb) != cudaSuccess) {
         cudaGetLastError();
         return QMOE_ERR_LAUNCH;
@@ -798,15 +811,28 @@ static int launch_pair(const Params &g, const uint8_t *w, const uint8_t *x, int6
     return launch_status();
 }
 
+template <int TN, typename T>
+static int launch_pair(const Params &p, const uint8_t *w, const uint8_t *x, int64_t bytes, cudaStream_t st, int dev, const DeviceInfo &di) {
+    if (p.epilogue == 0) return launch_pair<TN, T, 0>(p, w, x, bytes, st, dev, di);
+    if (p.epilogue == 1) return launch_pair<TN, T, 1>(p, w, x, bytes, st, dev, di);
+    return launch_pair<TN, T, 2>(p, w, x, bytes, st, dev, di);
+}
+
+// Up to 64 tokens: one tile of weight rows x all tokens per CTA, the stages split over a cluster where tiles are few. More:
+// pairs, with the columns that take the least time: waves of tiles times a tile's time, 1, 0.86 and 0.72 for 256, 192
+// and 128 columns (8192 x 12288 x 4096 in 155, 178 and 223 us). 2048 x 2688 x 4096: 19.6, 18.6, 23.0 us, 192 taken;
+// 128 x 4096 x 4096: 12.1, 11.5, 10.9, 128 taken (a cluster per tile of 128 x 128: 11.7).
 template <typename T>
 static int pick(const Params &p, const CUtensorMap &a, const uint8_t *w, const uint8_t *x, int64_t bytes, cudaStream_t st, int dev, const DeviceInfo &di) {
     if (p.M <= 16) return launch<16, T>(p, a, x, bytes, st, dev, di);
     if (p.M <= 32) return launch<32, T>(p, a, x, bytes, st, dev, di);
     if (p.M <= 64) return launch<64, T>(p, a, x, bytes, st, dev, di);
-    if (p.M <= 128 || (int64_t)p.nbn * ((p.M + 127) / 128) <= di.sms) return launch<128, T>(p, a, x, bytes, st, dev, di);
-    if (p.epilogue == 0) return launch_pair<256, T, 0>(p, w, x, bytes, st, dev, di);
-    if (p.epilogue == 1) return launch_pair<256, T, 1>(p, w, x, bytes, st, dev, di);
-    return launch_pair<256, T, 2>(p, w, x, bytes, st, dev, di);
+    const int64_t A = tokens_on_lanes<T>(p) ? p.M : p.N, B = tokens_on_lanes<T>(p) ? p.N : p.M, pairs = di.sms / 2;
+    auto cost = [&](int tn, int each) { return ((A + 255) / 256 * ((B + tn - 1) / tn) + pairs - 1) / pairs * each; };
+    const int64_t c128 = cost(128, 72), c192 = cost(192, 86), c256 = cost(256, 100);
+    if (c128 <= c192 && c128 <= c256) return launch_pair<128, T>(p, w, x, bytes, st, dev, di);
+    if (c192 <= c256) return launch_pair<192, T>(p, w, x, bytes, st, dev, di);
+    return launch_pair<256, T>(p, w, x, bytes, st, dev, di);
 }
 
 } // namespace g4
@@ -853,25 +879,6 @@ int dq_gemm_nvfp4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int
     if (y_dtype == QMOE_DT_BF16) return g4::pick<__nv_bfloat16>(p, a, w, x, K / 2, st, dev, *di);
     if (y_dtype == QMOE_DT_F16) return g4::pick<__half>(p, a, w, x, K / 2, st, dev, *di);
     return g4::pick<float>(p, a, w, x, K / 2, st, dev, *di);
-}
-
-size_t dq_linear_a4_workspace_bytes(int64_t M, int64_t K) {
-    if (M < 1 || M > (1 << 24) || K < 32 || (K % 32) || K > (1 << 24)) return 0;
-    return (size_t)(M * (K / 2) + (M + 127) / 128 * ((K + 63) / 64) * g4::ATOM + (M + 3) / 4 * 16 + M * (K / 16));
-}
-
-int dq_linear_a4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int sw_per_row, const void *x, int x_dtype,
-                 int64_t ldx, int M, int N, int K, int epilogue, const void *residual, void *y, void *workspace,
-                 size_t workspace_bytes, void *stream) {
-    if (!w || !w_atoms || !sw || !x || !y || !workspace || (epilogue == 2 && !residual)) return QMOE_ERR_NULL;
-    const size_t need = dq_linear_a4_workspace_bytes(M, K);
-    if (!need || N < 1 || N > (1 << 24) || epilogue < 0 || epilogue > 2) return QMOE_ERR_SHAPE;
-    if (!aligned16(workspace)) return QMOE_ERR_ALIGN;
-    if (workspace_bytes < need) return QMOE_ERR_WORKSPACE;
-    uint8_t *codes = static_cast<uint8_t *>(workspace), *atoms = codes + (int64_t)M * (K / 2);
-    uint8_t *s = atoms + (int64_t)((M + 127) / 128) * ((K + 63) / 64) * g4::ATOM, *sc = s + (int64_t)(M + 3) / 4 * 16;
-    if (int e = dq_quantize_nvfp4(x, x_dtype, ldx, M, K, 1, codes, sc, reinterpret_cast<float *>(s), atoms, stream)) return e;
-    return dq_gemm_nvfp4(w, w_atoms, sw, sw_per_row, codes, atoms, reinterpret_cast<float *>(s), 1, M, N, K, epilogue, residual, y, x_dtype, stream);
 }
 
 int dq_gemm_nvfp4_status(int clear, void *stream) {

@@ -276,7 +276,7 @@ __device__ __forceinline__ void choose(const Route &a, int64_t t, int lane, uint
         }
 }
 
-template <typename T, int EPL> __global__ void __launch_bounds__(THREADS) route_kernel(const Route a) {
+template <typename T, int EPL> __global__ void __launch_bounds__(THREADS, EPL > 16 ? 2 : 4) route_kernel(const Route a) {
     extern __shared__ float sm[];
     __shared__ uint4 cands[WARPS][MAX_CAND];
     int *hist = reinterpret_cast<int *>(sm);
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(1024) __cluster_dims__(FIN, 1, 1) balance_fina
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, int EPL> __global__ void __launch_bounds__(THREADS) balance_backward_kernel(const Balance a) {
+template <typename T, int EPL> __global__ void __launch_bounds__(THREADS, EPL > 16 ? 2 : 4) balance_backward_kernel(const Balance a) {
     const int lane = threadIdx.x & 31;
     const float g = *a.grad;
     float c[EPL];

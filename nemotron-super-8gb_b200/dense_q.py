@@ -283,12 +283,14 @@ def qlinear_a4(q, x, act=None, residual=None):
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
     if M and N:
         q = prepare(q)
-        n = M * (K // 2) + _atoms_bytes(M, K) + (M + 3) // 4 * 16 + M * (K // 16)   # dq_linear_a4_workspace_bytes
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        n, ws = 0, None
+        if M > 4 or K > 16384:
+            n = M * (K // 2) + _atoms_bytes(M, K) + (M + 3) // 4 * 16 + M * (K // 16)   # dq_linear_a4_workspace_bytes
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
         with _on(x):
-            C.call("dq_linear_a4", q["w"].data_ptr(), q["sca"].data_ptr(), q["s"].data_ptr(), int(q["fmt"] == "nvfp4_rows"),
+            C.call("dq_linear_a4", q["w"].data_ptr(), q["sc"].data_ptr(), q["sca"].data_ptr(), q["s"].data_ptr(), int(q["fmt"] == "nvfp4_rows"),
                    x.data_ptr(), dt, ld, M, N, K, ep, residual.data_ptr() if residual is not None else None, y.data_ptr(),
-                   ws.data_ptr(), n, C.stream_of(x))
+                   ws.data_ptr() if ws is not None else None, n, C.stream_of(x))
     return y if len(sh) == 2 else y.view(*sh[:-1], N)
 
 

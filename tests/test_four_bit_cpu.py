@@ -94,15 +94,15 @@ def test_python_refusals():
 
 def test_linear_arguments(lib):
     a = P(256)
-    need = lib.dq_linear_a4_workspace_bytes(4, 64)
-    assert need == 4 * 32 + 512 + 16 + 4 * 4
+    need = lib.dq_linear_a4_workspace_bytes(5, 64)
+    assert need == 5 * 32 + 512 + 32 + 5 * 4
     assert lib.dq_linear_a4_workspace_bytes(0, 64) == 0 and lib.dq_linear_a4_workspace_bytes(4, 48) == 0
 
-    def call(w=a, x=a, dt=1, ldx=64, M=4, N=8, K=64, ep=0, res=None, y=a, ws=a, n=need):
-        return lib.dq_linear_a4(w, a, a, 0, x, dt, ldx, M, N, K, ep, res, y, ws, n, None)
+    def call(w=a, x=a, dt=1, ldx=64, M=5, N=8, K=64, ep=0, res=None, y=a, ws=a, n=need):
+        return lib.dq_linear_a4(w, a, a, a, 0, x, dt, ldx, M, N, K, ep, res, y, ws, n, None)
 
     assert call(w=None) == 5 and call(x=None) == 5 and call(y=None) == 5 and call(ws=None) == 5 and call(ep=2) == 5
     assert call(M=0) == 1 and call(N=0) == 1 and call(K=16) == 1 and call(ep=3) == 1 and call(ldx=63) == 1
     assert call(ws=P(264)) == 2 and call(n=need - 1) == 8 and call(dt=9) == 6
     if not torch.cuda.is_available():
-        assert call() == 7
+        assert call() == 7 and call(M=4, ws=None, n=0) == 7    # few rows need no workspace

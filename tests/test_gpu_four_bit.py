@@ -300,3 +300,26 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right():
             Q.set_wait_cycles(0)
         assert D.gemm_status() == 0
         assert torch.equal(D.gemm(q, xq, torch.float32), ref) and D.gemm_status() == 0
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("N,K", [(1, 32), (3, 64), (17, 992), (2688, 4096), (300, 2080), (129, 16384), (100, 16416)])
+def test_linear_of_few_tokens(M, N, K):
+    """The one-kernel form (up to four rows) and the sizes beside it: the quantiser's own codes, strided rows, per-row
+    weight scales, a NaN block and a row of zeros."""
+    import dense_q as D
+    g = seeded(M * K + N)
+    q = D.prepare(D.quantize(torch.randn(N, K, generator=g, device=DEV) * 0.05, per_row=M % 2 == 0))
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        base = torch.randn(M, K + 8, generator=g, device=DEV).to(dtype)
+        for x in (base[:, :K], base[:, 3:3 + K]):
+            xq = D.quantize(x)
+            ref = values_of(xq) @ values_of(q).t()
+            y = D.qlinear_a4(q, x)
+            assert bool(((y.double() - ref).abs() <= bound(xq, q, y)).all())
+            assert torch.equal(D.qlinear_a4(q, x, act="relu2"), (torch.relu(y.float()) ** 2).to(dtype))
+        x = base[:, :K].clone()
+        x[M - 1] = 0
+        x[0, 5] = float("nan")
+        y = D.qlinear_a4(q, x)
+        assert torch.isnan(y[0]).all() and torch.isfinite(y[1:]).all() and (M == 1 or not y[M - 1].any())
