@@ -387,6 +387,16 @@ __device__ __forceinline__ void sigmoid_pair(float x, float &s, float &r) {
     r = e * s;
 }
 
+// Whether a row's p are its softmax: asked for, or scores so low (all under 2e-9) that sigmoid(x) is e^x to fp32's last
+// place. Their sigmoids may all underflow, their ratios need not.
+template <int EPL> __device__ __forceinline__ bool as_softmax(const float (&x)[EPL], bool softmax) {
+    if (softmax) return true;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < EPL; i++) m = fmaxf(m, x[i]);
+    return warp_max(m) < -20.f;
+}
+
 template <typename T, int EPL> __global__ void __launch_bounds__(BAL_THREADS) balance_kernel(const Balance a) {
     extern __shared__ float sm[];
     int *hist = reinterpret_cast<int *>(sm);              // [ne + 1]
@@ -408,7 +418,7 @@ template <typename T, int EPL> __global__ void __launch_bounds__(BAL_THREADS) ba
             if (e >= 0 && e < a.ne) atomicAdd(&hist[e], 1);
         }
         float inv = 1.f;
-        if (a.softmax) {
+        if (as_softmax<EPL>(s, a.softmax)) {
             softmax_row<EPL>(s, a.ne, lane);
         } else {
             float total = 0.f, r;
@@ -514,18 +524,19 @@ template <typename T, int EPL> __global__ void __launch_bounds__(THREADS, EPL > 
         }
         load_row<T, EPL>(static_cast<const T *>(a.logits) + t * a.ld, a.ne, lane, a.vec, s);
         float r[EPL], total = 0.f, dot = 0.f;
-        if (a.softmax) softmax_row<EPL>(s, a.ne, lane);
+        const bool soft = as_softmax<EPL>(s, a.softmax);
+        if (soft) softmax_row<EPL>(s, a.ne, lane);
 #pragma unroll
         for (int i = 0; i < EPL; i++) {
             r[i] = 1.f;
-            if (!a.softmax) {
+            if (!soft) {
                 sigmoid_pair(s[i], s[i], r[i]);
                 s[i] = expert<EPL>(i, lane) < a.ne ? s[i] : 0.f;
             }
             total += s[i];
             dot = fmaf(c[i], s[i], dot);
         }
-        const float inv = a.softmax ? 1.f : 1.f / warp_sum(total);
+        const float inv = soft ? 1.f : 1.f / warp_sum(total);
         dot = warp_sum(dot) * inv;
 #pragma unroll
         for (int i = 0; i < EPL; i++) s[i] = g * (s[i] * inv) * (c[i] - dot) * r[i];

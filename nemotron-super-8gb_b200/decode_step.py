@@ -15,6 +15,10 @@ NemotronHMoE.forward (tf:722-737) over device-side parts:
 static input/output buffers and replays it per token (one launch for the whole step). For one token on a
 T-layout store, everything after the router's fp32 linear (sigmoid, bias, top-k, weights and the store
 lookup of the chosen experts) is one kernel (qmoe_route_decode) instead of a dozen small torch launches.
+
+A prompt runs the same parts over its tokens. With `prompt_a4` its routing is one kernel too (router.route: the same
+experts and weights, in decreasing order of choice) and its NVFP4 linears take NVFP4 activations (dense_q.quantize and
+gemm) instead of dequantizing the weights for a bf16 product: faster, with the activations' four-bit rounding.
 """
 import torch
 import torch.nn.functional as F
@@ -22,6 +26,7 @@ import torch.nn.functional as F
 import _qmoe_lib as C
 import dense_q as D
 import qmoe_ns as Q
+import router as R
 from expert_store import RoutedExperts
 
 
@@ -63,14 +68,24 @@ def route_tokens(x, gate_w, bias, top_k=22, scaling=5.0, n_group=1, topk_group=1
     return ids, w * scaling
 
 
+def _four_bit(w):
+    """A weight the four-bit product takes."""
+    return isinstance(w, dict) and w["fmt"] == "nvfp4" and w["K"] % 32 == 0
+
+
 class MoELayer(torch.nn.Module):
     """One NemotronHMoE layer m (tf:663-737): gate_w [512, hidden] and bias [512] (router), fc1 [1024, hidden]
     and fc2 [hidden, 1024] (latent projections), shared_up [I, hidden] and shared_down [hidden, I] (shared
-    expert, relu^2), each a dense_q dict or a plain weight; the routed experts from `store`."""
+    expert, relu^2), each a dense_q dict or a plain weight; the routed experts from `store`. prompt_a4: more than
+    dense_q.MB_MAX tokens take the four-bit path (see above) for the NVFP4 weights among these; `counts` [512] int32
+    then holds how many of the last prompt's tokens chose each expert."""
 
     def __init__(self, m, store, gate_w, bias, fc1, fc2, shared_up, shared_down, top_k=22, scaling=5.0,
-                 n_group=1, topk_group=1, norm_topk_prob=False):
+                 n_group=1, topk_group=1, norm_topk_prob=False, prompt_a4=False):
         super().__init__()
+        self.prompt_a4, self.counts = prompt_a4, None
+        if prompt_a4:   # the weights' scales as the product reads them, once
+            fc1, fc2, shared_up, shared_down = (D.prepare(w) if _four_bit(w) else w for w in (fc1, fc2, shared_up, shared_down))
         self.gate_w = gate_w.to(torch.float32).contiguous()   # the router computes in fp32: convert once (exact)
         self.bias = bias.to(torch.float32).contiguous()
         self.fc1, self.fc2, self.shared_up, self.shared_down = fc1, fc2, shared_up, shared_down
@@ -104,6 +119,8 @@ class MoELayer(torch.nn.Module):
         x = hidden_states.reshape(-1, shape[-1])
         if self.fused and x.shape[0] == 1 and self._fused_shared(x, x):
             return self._forward_token(x).view(shape)
+        if self.prompt_a4 and x.shape[0] > D.MB_MAX:
+            return self._forward_prompt(x).view(shape)
         lat = linear(self.fc1, x)
         if self.fused and x.shape[0] == 1:
             _, coef, sidx, tab, s2 = self.route_decode(x)
@@ -127,6 +144,24 @@ class MoELayer(torch.nn.Module):
         u = torch.relu(linear(self.shared_up, x))
         out = out + linear(self.shared_down, u * u)
         return out.view(shape)
+
+    def _forward_prompt(self, x):
+        """More than MB_MAX tokens with four-bit activations: x is quantized once for fc1 and the shared up projection,
+        the squared ReLU and the last addition are the products' epilogues."""
+        logits = F.linear(x.to(torch.float32), self.gate_w)
+        ids, w, self.counts = R.route(logits, self.bias, **self.route_args)
+        xq = D.quantize(x, for_gemm=True) if _four_bit(self.fc1) or _four_bit(self.shared_up) else None
+        lat = D.gemm(self.fc1, xq, x.dtype) if _four_bit(self.fc1) else linear(self.fc1, x)
+        y = self.experts(lat, ids, w)
+        out = D.qlinear_a4(self.fc2, y) if _four_bit(self.fc2) else linear(self.fc2, y)
+        if _four_bit(self.shared_up):
+            u2 = D.gemm(self.shared_up, xq, x.dtype, act="relu2")
+        else:
+            u = torch.relu(linear(self.shared_up, x))
+            u2 = u * u
+        if _four_bit(self.shared_down):
+            return D.qlinear_a4(self.shared_down, u2, residual=out)
+        return out + linear(self.shared_down, u2)
 
     def _forward_token(self, x):
         """One token with every fused part: the latent projection fc1 and the whole shared expert (up projection

@@ -170,6 +170,8 @@ def _rows(x):
     C.ptr(x)
     dt = C.dtype_code(x)
     M, K = x.shape
+    if x.is_contiguous():
+        return x, dt, K
     if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
         x = x.contiguous()
     return x, dt, x.stride(0) if M > 1 else K
@@ -205,17 +207,26 @@ def quantize(x, per_row=True, for_gemm=False):
     return q
 
 
+_NVFP4 = ("nvfp4", "nvfp4_rows")
+
+
 def prepare(q):
     """A weight ready for gemm: the dict with "sca", its block scales as the tensor cores read them, added (the
     other tensors are shared with q)."""
-    if q["fmt"] not in ("nvfp4", "nvfp4_rows"):
+    if q["fmt"] not in _NVFP4:
         raise C.QmoeError(f"gemm takes NVFP4 weights (got {q['fmt']})")
     if "sca" in q:
         return q
     N, K = q["N"], q["K"]
+    for k, shape in (("w", (N, K // 2)), ("sc", (N, K // 16))):
+        if q[k].dtype != torch.uint8 or q[k].shape != shape or not q[k].is_contiguous():
+            raise C.QmoeError(f"{k} must be contiguous uint8 {list(shape)}")
+    if q["s"].dtype != torch.float32 or q["s"].numel() != (N if q["fmt"] == "nvfp4_rows" else 1) or not q["s"].is_contiguous():
+        raise C.QmoeError("s must be float32, one value (nvfp4) or one per row (nvfp4_rows)")
     if N == 0:
         return {**q, "sca": torch.empty(0, dtype=torch.uint8, device=q["sc"].device)}
-    sc = q["sc"].contiguous()
+    sc = q["sc"]
+    C.ptr(sc)
     sca = torch.empty(_atoms_bytes(N, K), dtype=torch.uint8, device=sc.device)
     with _on(sc):
         C.call("dq_scale_atoms", C.ptr(sc), N, K, C.ptr(sca), C.stream_of(sc))
@@ -223,7 +234,6 @@ def prepare(q):
 
 
 _ACTS = {None: 0, "relu2": 1}
-_NVFP4 = ("nvfp4", "nvfp4_rows")
 
 
 def _check_product(q, M, K, dtype, dev, act, residual):

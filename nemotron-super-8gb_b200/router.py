@@ -28,6 +28,8 @@ def _logits(x, score):
 
 def _rows(x):
     """x with unit column stride and rows that do not overlap, and its row stride."""
+    if x.is_contiguous():
+        return x, x.shape[1]
     if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         x = x.contiguous()
     return x, int(x.stride(0)) if x.shape[0] > 1 else x.shape[1]

@@ -106,3 +106,14 @@ def test_linear_arguments(lib):
     assert call(ws=P(264)) == 2 and call(n=need - 1) == 8 and call(dt=9) == 6
     if not torch.cuda.is_available():
         assert call() == 7 and call(M=4, ws=None, n=0) == 7    # few rows need no workspace
+
+
+def test_prepare_looks_at_the_weight():
+    import _qmoe_lib as C
+    import dense_q as D
+    q = {"fmt": "nvfp4", "w": torch.zeros(4, 32, dtype=torch.uint8), "sc": torch.zeros(4, 4, dtype=torch.uint8),
+         "s": torch.ones(1), "N": 4, "K": 64}
+    for bad in ({"w": torch.zeros(4, 31, dtype=torch.uint8)}, {"w": torch.zeros(4, 64, dtype=torch.uint8)[:, ::2]},
+                {"sc": torch.zeros(4, 4)}, {"s": torch.ones(4)}, {"s": torch.ones(1, dtype=torch.float64)}, {"fmt": "nvfp4_rows"}, {}):
+        with pytest.raises(C.QmoeError):
+            D.prepare({**q, **bad})

@@ -195,28 +195,37 @@ def loss64(x, ids, mask, score, coef):
 
 
 def check_balance(logits, ids, mask=None, score="sigmoid", coef=1.0):
+    """p from logarithms of the scores (log sigmoid(x) is x to 1e-13 below -30), so that none underflows, and the gradient
+    by its formula p_j (c_j - sum c p) (1 - s_j); test_training_step_of_both_and_reruns has it by automatic
+    differentiation, test_gradients_against_differences by differences."""
     import router as R
     leaf = logits.detach().clone().requires_grad_()
     loss, n = R.balance_loss(leaf, ids, mask, score, coef)
+    got, = torch.autograd.grad(loss * 3.0, leaf)
+    loss = loss.detach()
     x = logits.double()
-    if mask is not None:
-        x = torch.where(mask[:, None], x, 0.0)             # what masked rows hold does not matter
-    x.requires_grad_()
-    want, n64, c = loss64(x, ids, mask, score, coef)
+    keep = torch.ones(x.shape[0], dtype=torch.bool, device=DEV) if mask is None else mask
+    x = torch.where(keep[:, None], x, 0.0)                 # what masked rows hold does not matter
+    ls = x if score == "softmax" else torch.where(x < -30, x, -torch.log1p(torch.exp(-x)))
+    p = torch.where(keep[:, None], torch.exp(ls - torch.logsumexp(ls, -1, keepdim=True)), 0.0)
+    rows = int(keep.sum())
+    i = ids[keep].long().flatten()
+    n64 = torch.bincount(i[(i >= 0) & (i < x.shape[1])], minlength=x.shape[1])
+    f = n64.double() * x.shape[1] / (ids.shape[1] * max(rows, 1))
+    c = coef * f / max(rows, 1)
+    want = coef * (f * p.sum(0) / max(rows, 1)).sum()
     assert torch.equal(n, n64.to(torch.int32)) and loss.shape == () and loss.dtype == torch.float32
     assert abs(float(loss) - float(want)) <= TOL * abs(float(want))
-    got, = torch.autograd.grad(loss * 3.0, leaf)
-    ref, = torch.autograd.grad(want * 3.0, x)
-    s = torch.sigmoid(x) if score == "sigmoid" else torch.softmax(x, -1)
-    p = s / s.sum(-1, keepdim=True)
+    one_less = torch.sigmoid(-x) if score == "sigmoid" else 1.0
+    ref = 3 * p * (c - (c * p).sum(-1, keepdim=True)) * one_less
     half = torch.finfo(logits.dtype).eps / 2
     tiny = torch.finfo(logits.dtype).smallest_normal * torch.finfo(logits.dtype).eps
     size = 3 * p * (c + (c * p).sum(-1, keepdim=True))     # the two terms that are subtracted
     assert got.dtype == logits.dtype
-    assert bool(((got.double() - ref).abs() <= TOL * size + half * ref.abs() + tiny).all())
-    if mask is not None:
-        assert not got[~mask].any()
-    return loss.detach(), got
+    # 2^-90: in a row whose largest logit is -20 or more, a score below e^-87 counts as e^-87: p under e^-67 (96 bits down)
+    assert bool(((got.double() - ref).abs() <= TOL * size + half * ref.abs() + tiny + 2.0 ** -90 * (c + (c * p).sum(-1, keepdim=True))).all())
+    assert not got[~keep].any()
+    return loss, got
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -253,6 +262,36 @@ def test_balance_masks_and_odd_ids():
     import router as R
     loss, n = R.balance_loss(x[:0], ids[:0])
     assert float(loss) == 0.0 and not n.any()
+
+
+def test_balance_of_extreme_logits():
+    """Rows so low that every sigmoid underflows keep their ratios; large logits, and an expert ruled out by -inf or the
+    lowest number, have p = 0 there."""
+    g = seeded(61)
+    x = torch.randn(40, 96, generator=g, device=DEV)
+    x[:8] -= 30
+    x[8:16] -= 120
+    x[16:24] -= 3000
+    x[24:32] += 100
+    ids = torch.topk(x, 4)[1]
+    check_balance(x[:24], ids[:24])
+    check_balance(x[24:], ids[24:])
+    y = x[32:].clone()
+    y[:, 5] = -float("inf")
+    y[:, 7] = torch.finfo(torch.float32).min
+    for score in ("sigmoid", "softmax"):
+        _, grad = check_balance(y, ids[32:], None, score)
+        assert float(grad[:, [5, 7]].abs().max()) < 1e-30
+
+
+def test_second_gradients_are_refused():
+    import router as R
+    x = torch.randn(8, 16, generator=seeded(3), device=DEV, requires_grad=True)
+    ids, w, _ = R.route(x, None, top_k=2)
+    for out in (w.sum(), R.balance_loss(x, ids)[0]):
+        first, = torch.autograd.grad(out, x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(first.sum(), x)
 
 
 def test_even_load_gives_one():
