@@ -4,6 +4,7 @@ The library is the only compute path: if it is missing, or the current CUDA devi
 sm_100 part, every call raises. There is no CPU or PyTorch fallback.
 """
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -66,6 +67,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_bind = None
 
 
 class QmoeError(RuntimeError):
@@ -85,6 +87,22 @@ def lib():
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+def bind():
+    """qmoe_torch.so: the library's operators as functions of torch tensors. Raises if it was not built."""
+    global _bind
+    if _bind is None:
+        path = os.path.join(HERE, "qmoe_torch.so")
+        if not os.path.exists(path):
+            raise QmoeError(f"{path} is missing: build it with qmoe_build.py (or __graft_entry__.build())")
+        lib()
+        spec = importlib.util.spec_from_file_location("qmoe_torch", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.set_error_class(QmoeError)
+        _bind = mod
+    return _bind
 
 
 def status_string(code):

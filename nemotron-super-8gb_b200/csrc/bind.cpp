@@ -1,0 +1,372 @@
+// The operators of dense_q's four-bit part and of router as functions of torch tensors, over the C entry points: argument
+// checks, outputs from torch's allocator, the current stream, and automatic differentiation.
+//
+// Small calls are bound by the host. The same calls from Python by ctypes, with a torch.autograd.Function, took 113 us
+// for a loss and its gradient of 200 tokens, 60 us of them in the Python parts of the function and in handing
+// its backward pass to the engine's thread; a single quantisation took 13 us.
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include "../../include/qmoe_b200.h"
+
+#include <optional>
+#include <sstream>
+#include <stdexcept>
+#include <string>
+#include <tuple>
+#include <vector>
+
+namespace py = pybind11;
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+namespace {
+
+struct Refused : std::runtime_error { using std::runtime_error::runtime_error; };
+
+template <typename... A> [[noreturn]] void refuse(const A &...a) {
+    std::ostringstream s;
+    (s << ... << a);
+    throw Refused(s.str());
+}
+
+#define REQUIRE(cond, ...) \
+    do {                   \
+        if (!(cond)) refuse(__VA_ARGS__); \
+    } while (0)
+
+void status(int code, const char *name) {
+    REQUIRE(code == QMOE_OK, name, ": ", qmoe_status_string(code), " (status ", code, ")");
+}
+
+int dtype_code(at::ScalarType t) {
+    switch (t) {
+    case at::kFloat: return QMOE_DT_F32;
+    case at::kBFloat16: return QMOE_DT_BF16;
+    case at::kHalf: return QMOE_DT_F16;
+    default: return -1;
+    }
+}
+
+int activation(const Tensor &x) {
+    REQUIRE(x.is_cuda(), "libqmoe_b200 works on CUDA tensors only (got a CPU tensor)");
+    const int dt = dtype_code(x.scalar_type());
+    REQUIRE(dt >= 0, "unsupported activation dtype ", x.scalar_type());
+    return dt;
+}
+
+void *stream_of(const Tensor &x) { return c10::cuda::getCurrentCUDAStream(x.get_device()).stream(); }
+
+Tensor empty(at::IntArrayRef sizes, const Tensor &like, at::ScalarType t) { return at::empty(sizes, like.options().dtype(t).requires_grad(false)); }
+
+// A matrix as the kernels read it: unit column stride, rows that do not overlap; its row stride.
+Tensor rows_of(const Tensor &x, int64_t &ld) {
+    const int64_t M = x.size(0), K = x.size(1);
+    Tensor r = x.is_contiguous() || (x.stride(1) == 1 && (M <= 1 || x.stride(0) >= K)) ? x : x.contiguous();
+    ld = M > 1 ? r.stride(0) : K;
+    return r;
+}
+
+template <typename T = void> T *data(const OptTensor &t) { return t.has_value() && t->defined() ? static_cast<T *>(t->data_ptr()) : nullptr; }
+template <typename T = void> T *data(const Tensor &t) { return static_cast<T *>(t.data_ptr()); }
+
+// ------------------------------------------------------------------------------------------ four bits
+void no_grad(const Tensor &t) {
+    REQUIRE(!(t.requires_grad() && at::GradMode::is_enabled()), "the four-bit operators have no gradient: call them under torch.no_grad()");
+}
+
+// The tensors of a quantised matrix [N, K], as the kernels read them.
+void check_tensors(const Tensor &w, const Tensor &sc, const Tensor &s, bool per_row, int64_t N, int64_t K) {
+    for (auto [name, t, width] : {std::make_tuple("w", &w, K / 2), std::make_tuple("sc", &sc, K / 16)})
+        REQUIRE(t->scalar_type() == at::kByte && t->dim() == 2 && t->size(0) == N && t->size(1) == width && t->is_contiguous(),
+                name, " must be contiguous uint8 [", N, ", ", width, "]");
+    REQUIRE(s.scalar_type() == at::kFloat && s.numel() == (per_row ? N : 1) && s.is_contiguous(),
+            "s must be float32, one value (nvfp4) or one per row (nvfp4_rows)");
+    REQUIRE(w.is_cuda() && sc.device() == w.device() && s.device() == w.device(), "libqmoe_b200 works on CUDA tensors only, all of a weight on one device");
+}
+
+int64_t atoms_bytes(int64_t rows, int64_t K) { return (rows + 127) / 128 * ((K + 63) / 64) * 512; }
+
+Tensor scale_atoms(const Tensor &w, const Tensor &sc, const Tensor &s, bool per_row, int64_t N, int64_t K) {
+    check_tensors(w, sc, s, per_row, N, K);
+    const c10::cuda::CUDAGuard guard(sc.device());
+    const Tensor atoms = empty({atoms_bytes(N, K)}, sc, at::kByte);
+    if (N) status(dq_scale_atoms(data<uint8_t>(sc), N, K, data<uint8_t>(atoms), stream_of(sc)), "dq_scale_atoms");
+    return atoms;
+}
+
+py::tuple quantize(const Tensor &x0, bool per_row, bool for_gemm) {
+    REQUIRE(x0.dim() == 2, "quantize takes a matrix [M, K]");
+    const int64_t M = x0.size(0), K = x0.size(1);
+    REQUIRE(K >= 16 && K % 16 == 0, "quantize takes rows of a positive multiple of 16 elements (got ", K, ")");
+    REQUIRE(M > 0 || per_row, "a tensor without rows has no scale");
+    no_grad(x0);
+    const int dt = activation(x0);
+    int64_t ld;
+    const Tensor x = rows_of(x0, ld);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor w = empty({M, K / 2}, x, at::kByte), sc = empty({M, K / 16}, x, at::kByte), s = empty({per_row ? M : 1}, x, at::kFloat);
+    OptTensor atoms;
+    if (for_gemm) atoms = empty({atoms_bytes(M, K)}, x, at::kByte);
+    if (M)
+        status(dq_quantize_nvfp4(data(x), dt, ld, M, K, per_row, data<uint8_t>(w), data<uint8_t>(sc), data<float>(s), data<uint8_t>(atoms),
+                                 stream_of(x)), "dq_quantize_nvfp4");
+    return py::make_tuple(w, sc, s, atoms);
+}
+
+Tensor dequant(const Tensor &w, const Tensor &sc, const Tensor &s, bool per_row, int64_t N, int64_t K) {
+    REQUIRE(w.is_cuda(), "libqmoe_b200 works on CUDA tensors only (got a CPU tensor)");
+    const c10::cuda::CUDAGuard guard(w.device());
+    const Tensor out = empty({N, K}, w, at::kBFloat16);
+    if (N && per_row) status(dq_dequant_nvfp4(data<uint8_t>(w), data<uint8_t>(sc), data<float>(s), 1, N, K, 0, N, data(out), QMOE_DT_BF16, stream_of(w)), "dq_dequant_nvfp4");
+    else if (N) status(dq_dequant_rows(1, data<uint8_t>(w), data<uint8_t>(sc), data<float>(s), N, K, 0, N, data(out), QMOE_DT_BF16, stream_of(w)), "dq_dequant_rows");
+    return out;
+}
+
+// The epilogue's code, and the residual as the kernels read it.
+int epilogue(const std::optional<std::string> &act, OptTensor &residual, int64_t M, int64_t N, at::ScalarType dtype, at::Device dev) {
+    REQUIRE(!act || *act == "relu2", "gemm: act is None or 'relu2', and not together with a residual");
+    if (!residual) return act ? 1 : 0;
+    REQUIRE(!act, "gemm: act is None or 'relu2', and not together with a residual");
+    no_grad(*residual);
+    REQUIRE(residual->dim() == 2 && residual->size(0) == M && residual->size(1) == N && residual->scalar_type() == dtype && residual->device() == dev,
+            "gemm: the residual is [M, N] in the output's dtype, on its device");
+    residual = residual->contiguous();
+    return 2;
+}
+
+void check_weight(const Tensor &w, int64_t N, int64_t Kw, int64_t K, at::Device dev) {
+    REQUIRE(Kw == K, "gemm: ", K, " elements per activation row, ", Kw, " per weight row");
+    REQUIRE(K > 0 && K % 32 == 0, "gemm takes rows of a positive multiple of 32 elements (got ", K, ")");
+    REQUIRE(w.device() == dev, "gemm: weight on ", w.device(), ", activations on ", dev);
+    REQUIRE(N <= (1 << 24), "gemm: at most 2^24 weight rows");
+}
+
+Tensor gemm(const Tensor &w, const Tensor &wsc, OptTensor watoms, const Tensor &ws, bool w_rows, int64_t N, int64_t Kw, const Tensor &x, const Tensor &xsc,
+            OptTensor xatoms, const Tensor &xs, bool x_rows, int64_t M, int64_t K, at::ScalarType dtype, const std::optional<std::string> &act, OptTensor residual) {
+    REQUIRE(dtype_code(dtype) >= 0, "unsupported output dtype ", dtype);
+    check_weight(w, N, Kw, K, x.device());
+    const int ep = epilogue(act, residual, M, N, dtype, x.device());
+    REQUIRE(x.is_cuda(), "libqmoe_b200 works on CUDA tensors only (got a CPU tensor)");
+    REQUIRE(M <= (1 << 24), "gemm: at most 2^24 rows");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor y = empty({M, N}, x, dtype);
+    if (M && N) {
+        if (!watoms) watoms = scale_atoms(w, wsc, ws, w_rows, N, K);
+        if (!xatoms) xatoms = scale_atoms(x, xsc, xs, x_rows, M, K);
+        status(dq_gemm_nvfp4(data<uint8_t>(w), data<uint8_t>(watoms), data<float>(ws), w_rows, data<uint8_t>(x), data<uint8_t>(xatoms), data<float>(xs),
+                             x_rows, (int)M, (int)N, (int)K, ep, data(residual), data(y), dtype_code(dtype), stream_of(x)), "dq_gemm_nvfp4");
+    }
+    return y;
+}
+
+Tensor linear_a4(const Tensor &w, const Tensor &sc, OptTensor atoms, const Tensor &s, bool w_rows, int64_t N, int64_t Kw, const Tensor &x0,
+                 const std::optional<std::string> &act, OptTensor residual) {
+    REQUIRE(x0.dim() >= 1, "a linear takes rows [..., K]");
+    const int64_t K = x0.size(-1);
+    no_grad(x0);
+    const int dt = activation(x0);
+    int64_t ld;
+    const Tensor x = rows_of(x0.dim() == 2 ? x0 : x0.reshape({K ? x0.numel() / K : 0, K}), ld);
+    const int64_t M = x.size(0);
+    check_weight(w, N, Kw, K, x.device());
+    if (residual) residual = residual->reshape({-1, N});
+    const int ep = epilogue(act, residual, M, N, x.scalar_type(), x.device());
+    const c10::cuda::CUDAGuard guard(x.device());
+    std::vector<int64_t> shape = x0.sizes().vec();
+    shape.back() = N;
+    const Tensor y = empty(shape, x, x.scalar_type());
+    if (M && N) {
+        REQUIRE(M <= (1 << 24), "gemm: at most 2^24 rows");
+        if (!atoms) atoms = scale_atoms(w, sc, s, w_rows, N, K);
+        OptTensor ws;
+        const size_t n = M > 4 || K > 16384 ? dq_linear_a4_workspace_bytes(M, K) : 0;   // few rows need none
+        if (n) ws = empty({(int64_t)n}, x, at::kByte);
+        status(dq_linear_a4(data<uint8_t>(w), data<uint8_t>(sc), data<uint8_t>(atoms), data<float>(s), w_rows, data(x), dt, ld, (int)M, (int)N, (int)K, ep,
+                            data(residual), data(y), data(ws), n, stream_of(x)), "dq_linear_a4");
+    }
+    return y;
+}
+
+// ------------------------------------------------------------------------------------------ router
+int score_code(const std::string &score) {
+    REQUIRE(score == "sigmoid" || score == "softmax", "score is 'sigmoid' or 'softmax' (got '", score, "')");
+    return score == "softmax";
+}
+
+int check_logits(const Tensor &x) {
+    REQUIRE(x.dim() == 2 && x.size(1) >= 1 && x.size(1) <= 1024, "logits must be [T, E] with 1 <= E <= 1024 (got ", x.sizes(), ")");
+    return activation(x);
+}
+
+// A gradient that was asked for as part of a graph: a second differentiation through it is refused.
+Tensor once(const Tensor &g) {
+    if (!at::GradMode::is_enabled()) return g;
+    Tensor v = g.detach();
+    v.requires_grad_(true);
+    auto f = std::make_shared<torch::autograd::DelayedError>("the router's operators are differentiable once", 1);
+    return (*f)({v})[0];
+}
+
+struct RouteArgs { int64_t k, n_group, topk_group; bool norm; int score; double scaling; };
+
+std::tuple<Tensor, Tensor, Tensor> run_route(const Tensor &x0, const OptTensor &bias, const RouteArgs &a) {
+    int64_t ld;
+    const Tensor x = rows_of(x0, ld);
+    const int64_t T = x.size(0), E = x.size(1);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor ids = empty({T, a.k}, x, at::kLong), w = empty({T, a.k}, x, at::kFloat);
+    const Tensor n = T ? empty({E}, x, at::kInt) : at::zeros({E}, x.options().dtype(at::kInt).requires_grad(false));
+    if (T)
+        status(qmoe_route(data(x), dtype_code(x.scalar_type()), ld, data<float>(bias), T, (int)E, (int)a.k, (int)a.n_group, (int)a.topk_group, a.norm, a.score,
+                          (float)a.scaling, data<int64_t>(ids), data<float>(w), data<int32_t>(n), stream_of(x)), "qmoe_route");
+    return {ids, w, n};
+}
+
+struct Route : torch::autograd::Function<Route> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &logits, const OptTensor &bias, int64_t k,
+                                                  int64_t n_group, int64_t topk_group, bool norm, int64_t score, double scaling) {
+        auto [ids, w, n] = run_route(logits, bias, {k, n_group, topk_group, norm, (int)score, scaling});
+        ctx->save_for_backward({logits, ids});
+        ctx->saved_data["norm"] = norm;
+        ctx->saved_data["score"] = score;
+        ctx->saved_data["scaling"] = scaling;
+        ctx->mark_non_differentiable({ids, n});
+        ctx->set_materialize_grads(false);
+        return {ids, w, n};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(8);
+        if (!grads[1].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        int64_t ld;
+        const Tensor x = rows_of(saved[0], ld), &ids = saved[1];
+        const c10::cuda::CUDAGuard guard(x.device());
+        const Tensor dl = empty(x.sizes(), x, x.scalar_type());
+        if (x.size(0)) {
+            const Tensor dw = grads[1].to(at::kFloat).contiguous();
+            status(qmoe_route_backward(data(x), dtype_code(x.scalar_type()), ld, x.size(0), (int)x.size(1), (int)ids.size(1), ctx->saved_data["norm"].toBool(),
+                                       (int)ctx->saved_data["score"].toInt(), (float)ctx->saved_data["scaling"].toDouble(), data<int64_t>(ids),
+                                       data<float>(dw), data(dl), stream_of(x)), "qmoe_route_backward");
+        }
+        out[0] = once(dl);
+        return out;
+    }
+};
+
+py::tuple route(const Tensor &logits, OptTensor bias, int64_t top_k, double scaling, int64_t n_group, int64_t topk_group, bool norm, const std::string &score) {
+    const int sc = score_code(score);
+    check_logits(logits);
+    const int64_t E = logits.size(1);
+    REQUIRE(top_k >= 1 && top_k <= std::min<int64_t>(32, E), "top_k must lie in 1..", std::min<int64_t>(32, E), " (got ", top_k, ")");
+    REQUIRE(n_group >= 1 && n_group <= 32 && E % n_group == 0 && topk_group >= 1 && topk_group <= n_group && (n_group == 1 || E / n_group >= 2),
+            E, " experts do not split into ", n_group, " groups of two or more, ", topk_group, " of them kept");
+    if (bias) {
+        REQUIRE(sc == 0, "a softmax router takes no bias");
+        REQUIRE(bias->dim() == 1 && bias->size(0) == E && bias->device() == logits.device(), "bias must be [E], on the logits' device");
+        bias = bias->detach().to(at::kFloat).contiguous();
+    }
+    if (logits.requires_grad() && at::GradMode::is_enabled()) {
+        const auto r = Route::apply(logits, bias, top_k, n_group, topk_group, norm, (int64_t)sc, scaling);
+        return py::make_tuple(r[0], r[1], r[2]);
+    }
+    auto [ids, w, n] = run_route(logits, bias, {top_k, n_group, topk_group, norm, sc, scaling});
+    return py::make_tuple(ids, w, n);
+}
+
+// Loss, counts, and coef * f / T' per expert for the backward pass.
+std::tuple<Tensor, Tensor, Tensor> run_balance(const Tensor &x0, const Tensor &ids, const OptTensor &mask, int score, double coef) {
+    int64_t ld;
+    const Tensor x = rows_of(x0, ld);
+    const int64_t T = x.size(0), E = x.size(1);
+    const c10::cuda::CUDAGuard guard(x.device());
+    if (!T) {
+        const auto f = x.options().dtype(at::kFloat).requires_grad(false);
+        return {at::zeros({}, f), at::zeros({E}, f.dtype(at::kInt)), at::zeros({E}, f)};
+    }
+    const Tensor loss = empty({}, x, at::kFloat), n = empty({E}, x, at::kInt), c = empty({E}, x, at::kFloat);
+    const int64_t bytes = (int64_t)qmoe_balance_workspace_bytes(T, (int)E);
+    const Tensor ws = empty({bytes}, x, at::kByte);
+    status(qmoe_balance(data(x), dtype_code(x.scalar_type()), ld, data(ids), ids.scalar_type() == at::kLong, data<uint8_t>(mask), T, (int)E,
+                        (int)ids.size(1), score, (float)coef, data<float>(loss), data<int32_t>(n), data<float>(c), data(ws), (size_t)bytes, stream_of(x)), "qmoe_balance");
+    return {loss, n, c};
+}
+
+struct Balance : torch::autograd::Function<Balance> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &logits, const Tensor &ids, const OptTensor &mask,
+                                                  int64_t score, double coef) {
+        auto [loss, n, c] = run_balance(logits, ids, mask, (int)score, coef);
+        ctx->save_for_backward({logits, c, mask ? *mask : Tensor()});
+        ctx->saved_data["score"] = score;
+        ctx->mark_non_differentiable({n});
+        ctx->set_materialize_grads(false);
+        return {loss, n};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(5);
+        if (!grads[0].defined()) return out;
+        const auto saved = ctx->get_saved_variables();
+        int64_t ld;
+        const Tensor x = rows_of(saved[0], ld);
+        const c10::cuda::CUDAGuard guard(x.device());
+        const Tensor dl = empty(x.sizes(), x, x.scalar_type());
+        if (x.size(0)) {
+            const Tensor g = grads[0].to(at::kFloat);
+            const OptTensor mask = saved[2].defined() ? OptTensor(saved[2]) : OptTensor();
+            status(qmoe_balance_backward(data(x), dtype_code(x.scalar_type()), ld, data<uint8_t>(mask), x.size(0), (int)x.size(1),
+                                         (int)ctx->saved_data["score"].toInt(), data<float>(saved[1]), data<float>(g), data(dl), stream_of(x)), "qmoe_balance_backward");
+        }
+        out[0] = once(dl);
+        return out;
+    }
+};
+
+py::tuple balance_loss(const Tensor &logits, const Tensor &ids0, OptTensor mask, const std::string &score, double coef) {
+    const int sc = score_code(score);
+    check_logits(logits);
+    const int64_t T = logits.size(0);
+    REQUIRE(ids0.dim() == 2 && ids0.size(0) == T && ids0.size(1) >= 1 && (ids0.scalar_type() == at::kLong || ids0.scalar_type() == at::kInt),
+            "ids must be int64 or int32 [T, k] with k >= 1");
+    REQUIRE(ids0.device() == logits.device(), "ids must be on the logits' device");
+    const Tensor ids = ids0.contiguous();
+    if (mask) {
+        REQUIRE(mask->dim() == 1 && mask->size(0) == T && mask->scalar_type() == at::kBool && mask->device() == logits.device(),
+                "mask must be bool [T], on the logits' device");
+        mask = mask->contiguous();
+    }
+    if (logits.requires_grad() && at::GradMode::is_enabled()) {
+        const auto r = Balance::apply(logits, ids, mask, (int64_t)sc, coef);
+        return py::make_tuple(r[0], r[1]);
+    }
+    auto [loss, n, c] = run_balance(logits, ids, mask, sc, coef);
+    return py::make_tuple(loss, n);
+}
+
+py::object error_class;
+
+} // namespace
+
+PYBIND11_MODULE(qmoe_torch, m) {
+    m.def("set_error_class", [](py::object c) { error_class = std::move(c); });
+    py::register_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const Refused &e) {
+            PyErr_SetString(error_class ? error_class.ptr() : PyExc_RuntimeError, e.what());
+        }
+    });
+    m.def("quantize", &quantize);
+    m.def("scale_atoms", &scale_atoms);
+    m.def("dequant", &dequant);
+    m.def("gemm", &gemm);
+    m.def("linear_a4", &linear_a4);
+    m.def("route", &route);
+    m.def("balance_loss", &balance_loss);
+    m.add_object("_cleanup", py::capsule([] { error_class = py::object(); }));
+}

@@ -74,7 +74,7 @@ def dequant_rows(q, r0, r1, out):
     sc = q.get("sc")
     if q["fmt"] == "nvfp4_rows":
         if r1 > r0:
-            with _on(out):
+            with torch.cuda.device(out.device):
                 C.call("dq_dequant_nvfp4", C.ptr(q["w"]), C.ptr(sc), C.ptr(q["s"]), 1, q["N"], q["K"], r0, r1, C.ptr(out),
                        C.dtype_code(out), C.stream_of(out))
         return out
@@ -85,6 +85,8 @@ def dequant_rows(q, r0, r1, out):
 
 def dequant(q):
     """dense_q.py:191-196: whole weight -> bf16 [N, K]."""
+    if q["fmt"] != "fp8":
+        return C.bind().dequant(q["w"], q["sc"], q["s"], q["fmt"] == "nvfp4_rows", q["N"], q["K"])
     out = torch.empty(q["N"], q["K"], dtype=torch.bfloat16, device=q["w"].device)
     return dequant_rows(q, 0, q["N"], out)
 
@@ -138,124 +140,31 @@ def attach(lin, q):
     lin.forward = types.MethodType(_fwd, lin)
 
 
-class _on:
-    """The tensor's device as the current one, for the launch (nothing to do where it is)."""
-    __slots__ = ("dev", "was")
-
-    def __init__(self, t):
-        self.dev = t.get_device()
-
-    def __enter__(self):
-        self.was = torch._C._cuda_getDevice()
-        if self.was != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *a):
-        if self.was != self.dev:
-            torch.cuda.set_device(self.was)
-
-
-def _atoms_bytes(rows, K):
-    return (rows + 127) // 128 * ((K + 63) // 64) * 512
-
-
-def _no_grad(t):
-    if t.requires_grad and torch.is_grad_enabled():
-        raise C.QmoeError("the four-bit operators have no gradient: call them under torch.no_grad()")
-
-
-def _rows(x):
-    """A matrix as the kernels read it: unit column stride, rows that do not overlap; its dtype code and row stride."""
-    _no_grad(x)
-    C.ptr(x)
-    dt = C.dtype_code(x)
-    M, K = x.shape
-    if x.is_contiguous():
-        return x, dt, K
-    if x.stride(1) != 1 or (M > 1 and x.stride(0) < K):
-        x = x.contiguous()
-    return x, dt, x.stride(0) if M > 1 else K
-
-
 def quantize(x, per_row=True, for_gemm=False):
     """x [M, K] (bf16, fp16 or fp32; K a multiple of 16; rows may be strided) -> quantized dict: codes "w" [M, K/2],
     block scales "sc" [M, K/16] (e4m3 bytes), "s" f32 [M] with fmt "nvfp4_rows" (per_row), or [1] with fmt "nvfp4"
     (one scale for the tensor: a weight of this module); with for_gemm also "sca", the scales as gemm reads them (what
     prepare adds, in the same pass). s is the smallest power of two with amax <= 2688 s, scales and codes the nearest, ties to even. A 16-element block that holds an
     infinity or a NaN reads back as NaN; the others are as if that value were zero."""
-    if x.dim() != 2:
-        raise C.QmoeError("quantize takes a matrix [M, K]")
-    M, K = x.shape
-    if K < 16 or K % 16:
-        raise C.QmoeError(f"quantize takes rows of a positive multiple of 16 elements (got {K})")
-    if M == 0 and not per_row:
-        raise C.QmoeError("a tensor without rows has no scale")
-    x, dt, ld = _rows(x)
-    dev = x.device
-    w = torch.empty(M, K // 2, dtype=torch.uint8, device=dev)
-    sc = torch.empty(M, K // 16, dtype=torch.uint8, device=dev)
-    s = torch.empty(M if per_row else 1, dtype=torch.float32, device=dev)
-    q = {"fmt": "nvfp4_rows" if per_row else "nvfp4", "w": w, "sc": sc, "s": s, "N": M, "K": K}
-    sca = None
+    w, sc, s, sca = C.bind().quantize(x, per_row, for_gemm)
+    q = {"fmt": "nvfp4_rows" if per_row else "nvfp4", "w": w, "sc": sc, "s": s, "N": x.shape[0], "K": x.shape[1]}
     if for_gemm:
-        q["sca"] = torch.empty(_atoms_bytes(M, K), dtype=torch.uint8, device=dev)
-        sca = q["sca"].data_ptr()
-    if M:
-        with _on(x):
-            C.call("dq_quantize_nvfp4", x.data_ptr(), dt, ld, M, K, int(per_row), w.data_ptr(), sc.data_ptr(), s.data_ptr(), sca,
-                   C.stream_of(x))
+        q["sca"] = sca
     return q
 
 
-_NVFP4 = ("nvfp4", "nvfp4_rows")
+def _nvfp4(q):
+    if q["fmt"] not in ("nvfp4", "nvfp4_rows"):
+        raise C.QmoeError(f"the four-bit product takes NVFP4 operands (got {q['fmt']})")
 
 
 def prepare(q):
     """A weight ready for gemm: the dict with "sca", its block scales as the tensor cores read them, added (the
     other tensors are shared with q)."""
-    if q["fmt"] not in _NVFP4:
-        raise C.QmoeError(f"gemm takes NVFP4 weights (got {q['fmt']})")
+    _nvfp4(q)
     if "sca" in q:
         return q
-    N, K = q["N"], q["K"]
-    for k, shape in (("w", (N, K // 2)), ("sc", (N, K // 16))):
-        if q[k].dtype != torch.uint8 or q[k].shape != shape or not q[k].is_contiguous():
-            raise C.QmoeError(f"{k} must be contiguous uint8 {list(shape)}")
-    if q["s"].dtype != torch.float32 or q["s"].numel() != (N if q["fmt"] == "nvfp4_rows" else 1) or not q["s"].is_contiguous():
-        raise C.QmoeError("s must be float32, one value (nvfp4) or one per row (nvfp4_rows)")
-    if N == 0:
-        return {**q, "sca": torch.empty(0, dtype=torch.uint8, device=q["sc"].device)}
-    sc = q["sc"]
-    C.ptr(sc)
-    sca = torch.empty(_atoms_bytes(N, K), dtype=torch.uint8, device=sc.device)
-    with _on(sc):
-        C.call("dq_scale_atoms", C.ptr(sc), N, K, C.ptr(sca), C.stream_of(sc))
-    return {**q, "sca": sca}
-
-
-_ACTS = {None: 0, "relu2": 1}
-
-
-def _check_product(q, M, K, dtype, dev, act, residual):
-    """The epilogue's code, and the residual as the kernels read it."""
-    if q["fmt"] not in _NVFP4:
-        raise C.QmoeError(f"gemm takes NVFP4 operands (got {q['fmt']})")
-    if q["K"] != K:
-        raise C.QmoeError(f"gemm: {K} elements per activation row, {q['K']} per weight row")
-    if K % 32 or K == 0:
-        raise C.QmoeError(f"gemm takes rows of a positive multiple of 32 elements (got {K})")
-    if act not in _ACTS or (act is not None and residual is not None):
-        raise C.QmoeError("gemm: act is None or 'relu2', and not together with a residual")
-    if dtype not in C.DT:
-        raise C.QmoeError(f"unsupported output dtype {dtype}")
-    if q["w"].device != dev:
-        raise C.QmoeError(f"gemm: weight on {q['w'].device}, activations on {dev}")
-    if residual is None:
-        return _ACTS[act], None
-    _no_grad(residual)
-    if residual.shape != (M, q["N"]) or residual.dtype != dtype or residual.device != dev:
-        raise C.QmoeError("gemm: the residual is [M, N] in the output's dtype, on its device")
-    return 2, residual.contiguous()
+    return {**q, "sca": C.bind().scale_atoms(q["w"], q["sc"], q["s"], q["fmt"] == "nvfp4_rows", q["N"], q["K"])}
 
 
 def gemm(q, xq, dtype=torch.bfloat16, act=None, residual=None):
@@ -263,45 +172,18 @@ def gemm(q, xq, dtype=torch.bfloat16, act=None, residual=None):
     either without "sca" has its scales laid out in this call), products exact, fp32 sums in a
     fixed order. act "relu2": relu(y)^2; residual [M, N] in dtype: y + residual; each on y rounded to dtype, as the
     unfused torch operators. K a multiple of 32."""
-    if xq["fmt"] not in _NVFP4:
-        raise C.QmoeError(f"gemm takes NVFP4 operands (got {xq['fmt']})")
-    M, N, K = xq["N"], q["N"], xq["K"]
-    dev = xq["w"].device
-    ep, residual = _check_product(q, M, K, dtype, dev, act, residual)
-    y = torch.empty(M, N, dtype=dtype, device=dev)
-    if M == 0 or N == 0:
-        return y
-    q, xq = prepare(q), prepare(xq)
-    with _on(y):
-        C.call("dq_gemm_nvfp4", C.ptr(q["w"]), C.ptr(q["sca"]), C.ptr(q["s"]), int(q["fmt"] == "nvfp4_rows"),
-               C.ptr(xq["w"]), C.ptr(xq["sca"]), C.ptr(xq["s"]), int(xq["fmt"] == "nvfp4_rows"), M, N, K, ep,
-               C.ptr(residual), C.ptr(y), C.DT[dtype], C.stream_of(y))
-    return y
+    _nvfp4(q)
+    _nvfp4(xq)
+    return C.bind().gemm(q["w"], q["sc"], q.get("sca"), q["s"], q["fmt"] == "nvfp4_rows", q["N"], q["K"], xq["w"], xq["sc"],
+                         xq.get("sca"), xq["s"], xq["fmt"] == "nvfp4_rows", xq["N"], xq["K"], dtype, act, residual)
 
 
 def qlinear_a4(q, x, act=None, residual=None):
     """qlinear with the activations in NVFP4 too: x [..., K] is quantized row by row, then multiplied as gemm does:
     [..., N] in x.dtype (residual of that shape). The result carries the activations' four-bit rounding (about a tenth
     of a row's norm) and takes a fraction of a bf16 product's time."""
-    sh = x.shape
-    K, N = sh[-1], q["N"]
-    x, dt, ld = _rows(x if len(sh) == 2 else x.reshape(-1, K))
-    M, dev = x.shape[0], x.device
-    if residual is not None:
-        residual = residual.reshape(-1, N)
-    ep, residual = _check_product(q, M, K, x.dtype, dev, act, residual)
-    y = torch.empty(M, N, dtype=x.dtype, device=dev)
-    if M and N:
-        q = prepare(q)
-        n, ws = 0, None
-        if M > 4 or K > 16384:
-            n = M * (K // 2) + _atoms_bytes(M, K) + (M + 3) // 4 * 16 + M * (K // 16)   # dq_linear_a4_workspace_bytes
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        with _on(x):
-            C.call("dq_linear_a4", q["w"].data_ptr(), q["sc"].data_ptr(), q["sca"].data_ptr(), q["s"].data_ptr(), int(q["fmt"] == "nvfp4_rows"),
-                   x.data_ptr(), dt, ld, M, N, K, ep, residual.data_ptr() if residual is not None else None, y.data_ptr(),
-                   ws.data_ptr() if ws is not None else None, n, C.stream_of(x))
-    return y if len(sh) == 2 else y.view(*sh[:-1], N)
+    _nvfp4(q)
+    return C.bind().linear_a4(q["w"], q["sc"], q.get("sca"), q["s"], q["fmt"] == "nvfp4_rows", q["N"], q["K"], x, act, residual)
 
 
 def gemm_status(device=None, clear=True):
