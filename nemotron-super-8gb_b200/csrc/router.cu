@@ -135,11 +135,10 @@ struct Route {
     void *dl;
 };
 
-// Order of choices as unsigned keys: larger choice, larger key; 0 is below every choice.
+// Order of choices (no NaN, no -0) as unsigned keys: larger choice, larger key; 0 is below every choice.
 __device__ __forceinline__ uint32_t key_of(float c) {
-    c = c != c ? -INFINITY : c + 0.f;   // + 0: the two zeros are equal
     const uint32_t b = __float_as_uint(c);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
 
 // Keeps the choices of the topk_group groups with the largest sums of their two best choices (ties to the lower group),
@@ -149,7 +148,7 @@ __device__ __forceinline__ void keep_groups(float (&c)[EPL], const Route &a, flo
     const int size = a.ne / a.n_group;
 #pragma unroll
     for (int i = 0; i < EPL; i++)
-        if (expert<EPL>(i, lane) < a.ne) buf[expert<EPL>(i, lane)] = c[i] != c[i] ? -INFINITY : c[i];
+        if (expert<EPL>(i, lane) < a.ne) buf[expert<EPL>(i, lane)] = c[i];
     __syncwarp();
     float mine = -INFINITY;   // lane g: group g's sum
     for (int g = 0; g < a.n_group; g++) {
@@ -179,134 +178,195 @@ __device__ __forceinline__ void keep_groups(float (&c)[EPL], const Route &a, flo
     __syncwarp();
 }
 
-// The lane's value of a descending bitonic sort of the warp's 32 keys.
-__device__ __forceinline__ uint32_t sort_desc(uint32_t v, int lane) {
+// The lane's value of a descending bitonic sort of the warp's 32 values.
+__device__ __forceinline__ float sort_desc(float v, int lane) {
 #pragma unroll
     for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll
         for (int j = k >> 1; j; j >>= 1) {
-            const uint32_t o = __shfl_xor_sync(0xffffffffu, v, j);
-            v = ((lane & j) == 0) == ((lane & k) == 0) ? max(v, o) : min(v, o);
+            const float o = __shfl_xor_sync(0xffffffffu, v, j);
+            v = ((lane & j) == 0) == ((lane & k) == 0) ? fmaxf(v, o) : fminf(v, o);
         }
     return v;
 }
 
 constexpr int MAX_CAND = 64;
+struct Candidates {   // of one warp: choice (as a key) and expert, the lower expert larger; score
+    unsigned long long key[MAX_CAND];
+    float s[MAX_CAND];
+};
 
-// One token. The k-th largest of the 32 lanes' largest keys bounds the k-th largest key from below, so only the keys
-// from there on can be chosen: about 34 for 512 experts and k = 22. They are gathered in shared memory, and the rank of
-// each among them, counted by a lane, is its place: (key, lower expert first) is unique. Rows with many equal keys, or
-// too few lanes with experts, can have more than MAX_CAND; those take k rounds of the warp's maximum. On random logits
-// of 16384 x 512 the rounds alone took 94 us.
-template <int EPL>
-__device__ __forceinline__ void choose(const Route &a, int64_t t, int lane, uint32_t (&key)[EPL], const float (&s)[EPL], uint4 *cand, int *hist) {
-    uint32_t top = 0;
+// k rounds of the warp's largest key, of equal ones the lowest expert: lane r gets the r-th. For rows with many equal
+// choices; on random logits of 16384 x 512 these rounds alone took 94 us. FAST: v holds logits, else scores, c choices.
+template <int EPL, bool FAST>
+__device__ __noinline__ void choose_by_rounds(const Route &a, int lane, const float (&c)[EPL], const float (&v)[EPL], const float *bias, int &id, float &sc) {
+    uint32_t key[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; i++) top = max(top, key[i]);
-    const uint32_t bound = max(__shfl_sync(0xffffffffu, sort_desc(top, lane), a.k - 1), 1u);
-    int cnt = 0;
+    for (int i = 0; i < EPL; i++) {
+        const int e = expert<EPL>(i, lane);
+        key[i] = e < a.ne ? key_of(FAST ? fmaxf(sigmoid(v[i]) + bias[e], -INFINITY) : c[i]) : 0u;
+    }
+    for (int r = 0; r < a.k; r++) {
+        uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < EPL; i++) cnt += key[i] >= bound;
+        for (int i = 0; i < EPL; i++) m = max(m, key[i]);
+        m = __reduce_max_sync(0xffffffffu, m);
+        uint32_t e = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = EPL - 1; i >= 0; i--)
+            if (key[i] == m) e = expert<EPL>(i, lane);
+        e = __reduce_min_sync(0xffffffffu, e);
+        float x = 0.f;
+        bool here = false;
+#pragma unroll
+        for (int i = 0; i < EPL; i++)
+            if (e == (uint32_t)expert<EPL>(i, lane)) {
+                key[i] = 0u;
+                x = v[i];
+                here = true;
+            }
+        x = __shfl_sync(0xffffffffu, x, __ffs(__ballot_sync(0xffffffffu, here)) - 1);
+        if (lane == r) id = (int)e, sc = FAST ? sigmoid(x) : x;
+    }
+}
+
+// One token. The k-th largest of the 32 lanes' largest choices bounds the k-th largest choice from below, so only those
+// from there on can be chosen: about 34 of 512 experts for k = 22. They are gathered in shared memory, and the rank of
+// each among them is its place, since (choice, lower expert first) is unique: a lane counts the rank of one, and what is
+// beyond 32 the warp counts by votes. More than MAX_CAND, or a bound of -inf: by rounds.
+//
+// FAST (sigmoid scores, no groups): c holds choices of approximate scores and v the logits. An approximate score is off by
+// under 2^-21 (its exponent's rounding, |x| 2^-24, shrinks by s (1 - s); two approximate instructions), so with twice
+// that and two places of the sum as a margin no choice at or above the bound is missed; torch's bits are computed for
+// the gathered ones alone. That took 1,580 instructions a token to 700.
+template <int EPL, bool FAST>
+__device__ __forceinline__ void choose(const Route &a, int64_t t, int lane, const float (&c)[EPL], const float (&v)[EPL], const float *bias, Candidates &cand, int *hist) {
+    float top = c[0];
+#pragma unroll
+    for (int i = 1; i < EPL; i++) top = fmaxf(top, c[i]);
+    float bound = __shfl_sync(0xffffffffu, sort_desc(top, lane), a.k - 1);
+    if (FAST) bound -= 4e-6f + fabsf(bound) * 0x1p-21f;
+    uint32_t in = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; i++) in |= (uint32_t)(c[i] >= bound) << i;
+    const int cnt = __popc(in);
     int off = cnt;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, off, o);
-        if (lane >= o) off += v;
+        const int u = __shfl_up_sync(0xffffffffu, off, o);
+        if (lane >= o) off += u;
     }
     const int n = __shfl_sync(0xffffffffu, off, 31);
     off -= cnt;
-    int id[2] = {0, 0}, rank[2] = {MAX_K, MAX_K};
-    float sc[2] = {0.f, 0.f};
-    if (n <= MAX_CAND) {
+    int id = 0, rank = MAX_K, id2 = 0, rank2 = MAX_K;
+    float sc = 0.f, sc2 = 0.f;
+    if (n <= MAX_CAND && bound > -INFINITY) {
 #pragma unroll
         for (int i = 0; i < EPL; i++)
-            if (key[i] >= bound) cand[off++] = make_uint4(~(uint32_t)expert<EPL>(i, lane), key[i], __float_as_uint(s[i]), 0u);
-        __syncwarp();
-        unsigned long long mine[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int c = lane + 32 * u;
-            mine[u] = ~0ull;   // none: ranks behind nothing, and is not stored
-            if (c < n) {
-                const uint4 v = cand[c];
-                mine[u] = (unsigned long long)v.y << 32 | v.x;
-                id[u] = (int)~v.x;
-                sc[u] = __uint_as_float(v.z);
-                rank[u] = 0;
+            if (in >> i & 1u) {
+                const uint32_t e = expert<EPL>(i, lane);
+                cand.key[off] = (FAST ? 0ull : (unsigned long long)key_of(c[i]) << 32) | (0xFFFFFFFFu - e);
+                cand.s[off++] = v[i];
             }
+        __syncwarp();
+        unsigned long long mine = ~0ull, mine2 = 0;
+        auto take = [&](int j, unsigned long long &key, int &e, float &score) {
+            key = cand.key[j];
+            e = (int)~(uint32_t)key;
+            score = cand.s[j];
+            if (FAST) {
+                score = sigmoid(score);
+                key |= (unsigned long long)key_of(fmaxf(score + bias[e], -INFINITY)) << 32;
+                cand.key[j] = key;
+            }
+        };
+        if (lane < n) {
+            take(lane, mine, id, sc);
+            rank = 0;
         }
-        for (int j = 0; j < n; j++) {
-            const unsigned long long v = *reinterpret_cast<const unsigned long long *>(&cand[j]);
-            rank[0] += v > mine[0];
-            if (n > 32) rank[1] += v > mine[1];
+        if (lane + 32 < n) take(lane + 32, mine2, id2, sc2);
+        if (lane == 0 && (n & 1)) cand.key[n] = 0;   // the loop takes two at a time; n odd is below MAX_CAND
+        __syncwarp();
+#pragma unroll 4
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(&cand.key[j]);
+            rank += u.x > mine;
+            rank += u.y > mine;
+        }
+        for (int j = 32; j < n; j++) {
+            const unsigned long long u = cand.key[j];
+            const int r = __popc(__ballot_sync(0xffffffffu, lane < n && mine > u)) + __popc(__ballot_sync(0xffffffffu, mine2 > u));
+            if (lane + 32 == j) rank2 = r;
         }
         __syncwarp();
     } else {
-        for (int r = 0; r < a.k; r++) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < EPL; i++) m = max(m, key[i]);
-            m = __reduce_max_sync(0xffffffffu, m);
-            uint32_t e = 0xFFFFFFFFu;
-#pragma unroll
-            for (int i = EPL - 1; i >= 0; i--)
-                if (key[i] == m) e = expert<EPL>(i, lane);
-            e = __reduce_min_sync(0xffffffffu, e);
-            float v = 0.f;
-            bool here = false;
-#pragma unroll
-            for (int i = 0; i < EPL; i++)
-                if (e == (uint32_t)expert<EPL>(i, lane)) {
-                    key[i] = 0u;
-                    v = s[i];
-                    here = true;
-                }
-            v = __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, here)) - 1);
-            if (lane == r) id[0] = (int)e, sc[0] = v, rank[0] = r;
-        }
+        choose_by_rounds<EPL, FAST>(a, lane, c, v, bias, id, sc);
+        if (lane < a.k) rank = lane;
     }
     float total = 1.f;
-    if (a.norm) total = warp_sum((rank[0] < a.k ? sc[0] : 0.f) + (rank[1] < a.k ? sc[1] : 0.f)) + 1e-20f;
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-        if (rank[u] < a.k) {
-            a.ids[t * a.k + rank[u]] = id[u];
-            a.w[t * a.k + rank[u]] = (a.norm ? sc[u] / total : sc[u]) * a.scaling;
-            atomicAdd(&hist[id[u]], 1);
-        }
+    if (a.norm) total = warp_sum((rank < a.k ? sc : 0.f) + (rank2 < a.k ? sc2 : 0.f)) + 1e-20f;
+    if (rank < a.k) {
+        a.ids[t * a.k + rank] = id;
+        a.w[t * a.k + rank] = (a.norm ? sc / total : sc) * a.scaling;
+        atomicAdd(&hist[id], 1);
+    }
+    if (rank2 < a.k) {
+        a.ids[t * a.k + rank2] = id2;
+        a.w[t * a.k + rank2] = (a.norm ? sc2 / total : sc2) * a.scaling;
+        atomicAdd(&hist[id2], 1);
+    }
 }
 
-template <typename T, int EPL> __global__ void __launch_bounds__(THREADS, EPL > 16 ? 2 : 4) route_kernel(const Route a) {
-    extern __shared__ float sm[];
-    __shared__ uint4 cands[WARPS][MAX_CAND];
-    int *hist = reinterpret_cast<int *>(sm);
-    float *buf = sm + a.ne + (threadIdx.x >> 5) * a.ne;   // only with groups
-    const int lane = threadIdx.x & 31;
-    for (int e = threadIdx.x; e < a.ne; e += THREADS) hist[e] = 0;
+// blockDim.x / 32 tokens at a time, up to ROUTE_WARPS. Every CTA adds its counts to the global ones at its end, so many
+// tokens take one large CTA per SM (16384 x 512: 29 us with four of eight warps), few tokens small ones on many SMs.
+template <int EPL> constexpr int ROUTE_WARPS = EPL > 16 ? 16 : 32;
+template <typename T, int EPL, bool FAST> __global__ void __launch_bounds__(ROUTE_WARPS<EPL> * 32) route_kernel(const Route a) {
+    constexpr int SLOTS = EPL * 32;
+    extern __shared__ __align__(16) uint8_t raw[];
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Candidates &cand = reinterpret_cast<Candidates *>(raw)[warp];
+    float *bias = reinterpret_cast<float *>(raw + warps * sizeof(Candidates));   // [SLOTS], 0 without one
+    int *hist = reinterpret_cast<int *>(bias + SLOTS);                           // [ne]
+    float *buf = reinterpret_cast<float *>(hist + a.ne) + warp * a.ne;           // [warps][ne], only with groups
+    for (int e = threadIdx.x; e < SLOTS; e += blockDim.x) {
+        bias[e] = a.bias && e < a.ne ? a.bias[e] : 0.f;
+        if (e < a.ne) hist[e] = 0;
+    }
     __syncthreads();
-    for (int64_t t = blockIdx.x * (int64_t)WARPS + (threadIdx.x >> 5); t < a.T; t += (int64_t)gridDim.x * WARPS) {
-        float s[EPL], c[EPL];
-        load_row<T, EPL>(static_cast<const T *>(a.logits) + t * a.ld, a.ne, lane, a.vec, s);
-        if (a.softmax) {
+    for (int64_t t = blockIdx.x * (int64_t)warps + warp; t < a.T; t += (int64_t)gridDim.x * warps) {
+        float v[EPL], c[EPL];   // logits (FAST) or scores; choices
+        load_row<T, EPL>(static_cast<const T *>(a.logits) + t * a.ld, a.ne, lane, a.vec, v);
+        if constexpr (FAST) {
 #pragma unroll
-            for (int i = 0; i < EPL; i++) c[i] = s[i];
-            softmax_row<EPL>(s, a.ne, lane);
+            for (int i = 0; i < EPL; i++) {
+                float e, s;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v[i] * -1.44269504f));
+                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+                c[i] = fmaxf(s + bias[expert<EPL>(i, lane)], -INFINITY);         // a NaN last
+            }
+        } else if (a.softmax) {
+#pragma unroll
+            for (int i = 0; i < EPL; i++) c[i] = fmaxf(v[i], -INFINITY) + 0.f;   // the two zeros are equal
+            softmax_row<EPL>(v, a.ne, lane);
         } else {
 #pragma unroll
             for (int i = 0; i < EPL; i++) {
-                const int e = expert<EPL>(i, lane);
-                s[i] = sigmoid(s[i]);
-                c[i] = a.bias && e < a.ne ? s[i] + a.bias[e] : s[i];
+                v[i] = sigmoid(v[i]);
+                c[i] = fmaxf(v[i] + bias[expert<EPL>(i, lane)], -INFINITY);      // no score is -0, so no choice is
             }
         }
-        if (a.n_group > 1) keep_groups<EPL>(c, a, a.softmax ? -INFINITY : 0.f, buf, lane);
-        uint32_t key[EPL];
+        if constexpr (!FAST)
+            if (a.n_group > 1) keep_groups<EPL>(c, a, a.softmax ? -INFINITY : 0.f, buf, lane);
+        if (a.ne < SLOTS)
 #pragma unroll
-        for (int i = 0; i < EPL; i++) key[i] = expert<EPL>(i, lane) < a.ne ? key_of(c[i]) : 0u;
-        choose<EPL>(a, t, lane, key, s, cands[threadIdx.x >> 5], hist);
+            for (int i = 0; i < EPL; i++)
+                if (expert<EPL>(i, lane) >= a.ne) c[i] = -INFINITY;
+        choose<EPL, FAST>(a, t, lane, c, v, bias, cand, hist);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < a.ne; e += THREADS) {   // integers: the order of the additions does not matter
+    const int turn = (int)(blockIdx.x * 96u % a.ne);   // CTAs that end together start at different experts
+    for (int i = threadIdx.x; i < a.ne; i += blockDim.x) {   // integers: the order of the additions does not matter
+        const int e = i + turn < a.ne ? i + turn : i + turn - a.ne;
         if (gridDim.x == 1) a.counts[e] = hist[e];
         else if (hist[e]) atomicAdd(&a.counts[e], hist[e]);
     }
@@ -377,73 +437,89 @@ struct Balance {
     void *dl;
 };
 
-constexpr int BAL_WARPS = 16, BAL_THREADS = BAL_WARPS * 32, MAX_PARTS = 320;
+constexpr int MAX_PARTS = 160;
+// A CTA per SM: 32 warps of 64 registers, 16 where a lane holds 32 experts.
+template <int EPL> constexpr int BAL_WARPS = EPL > 16 ? 16 : 32;
 
-// sigmoid and 1 - sigmoid as products of one reciprocal (1 ulp): neither loses digits near 1, and nothing is decided
-// by their last bit, as it is in the routing.
+// sigmoid and 1 - sigmoid as products of one reciprocal (1 ulp), where nothing is decided by their last bit, as it is in
+// the routing: neither loses digits near 1. e^-x is 2^y for y = fl(-x log2 e), corrected by what that rounding left.
+// x is kept to [-87, 126] (a NaN stays one), where all of it is a normal number; what lies outside counts as the border.
 __device__ __forceinline__ void sigmoid_pair(float x, float &s, float &r) {
-    const float e = fminf(expf(-x), 8e37f);   // its reciprocal is still a normal number
+    asm("max.NaN.f32 %0, %0, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(x));
+    constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
+    const float y = -x * LOG2E;
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+    e = fmaf(e, fmaf(-x, LOG2E, -y) * LN2, e);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
     r = e * s;
 }
 
-// Whether a row's p are its softmax: asked for, or scores so low (all under 2e-9) that sigmoid(x) is e^x to fp32's last
-// place. Their sigmoids may all underflow, their ratios need not.
-template <int EPL> __device__ __forceinline__ bool as_softmax(const float (&x)[EPL], bool softmax) {
-    if (softmax) return true;
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < EPL; i++) m = fmaxf(m, x[i]);
-    return warp_max(m) < -20.f;
-}
+// A row whose scores sum to less is under -20 everywhere: sigmoid(x) is e^x to fp32's last place there, and p the softmax.
+// Its sigmoids may all underflow, their ratios need not.
+constexpr float LOW = 2e-9f;
 
-template <typename T, int EPL> __global__ void __launch_bounds__(BAL_THREADS) balance_kernel(const Balance a) {
+template <typename T, int EPL> __global__ void __launch_bounds__(BAL_WARPS<EPL> * 32) balance_kernel(const Balance a) {
+    constexpr int W = BAL_WARPS<EPL>;
     extern __shared__ float sm[];
-    int *hist = reinterpret_cast<int *>(sm);              // [ne + 1]
-    float *sums = sm + a.ne + 1;                          // [ne]
+    float *sums = sm;                                     // [W][ne]
+    int *hist = reinterpret_cast<int *>(sm + W * a.ne);   // [ne + 1]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int e = threadIdx.x; e < 2 * a.ne + 1; e += BAL_THREADS) sm[e] = 0.f;   // zero bits for both
+    for (int e = threadIdx.x; e <= a.ne; e += W * 32) hist[e] = 0;
     __syncthreads();
     float acc[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; i++) acc[i] = 0.f;
     int rows = 0;
-    for (int64_t t = blockIdx.x * (int64_t)BAL_WARPS + warp; t < a.T; t += (int64_t)gridDim.x * BAL_WARPS) {
-        if (a.mask && !a.mask[t]) continue;
+    const int64_t step = (int64_t)gridDim.x * W;
+    uint32_t live = ~0u;   // masks of the warp's next 32 tokens, fetched together
+    int left = 0;
+    for (int64_t t = blockIdx.x * (int64_t)W + warp; t < a.T; t += step, live >>= 1, left--) {
+        if (a.mask && left == 0) {
+            live = __ballot_sync(0xffffffffu, t + lane * step < a.T && a.mask[t + lane * step]);
+            left = 32;
+        }
+        if (!(live & 1u)) continue;
         rows++;
+        const T *row = static_cast<const T *>(a.logits) + t * a.ld;
         float s[EPL];
-        load_row<T, EPL>(static_cast<const T *>(a.logits) + t * a.ld, a.ne, lane, a.vec, s);
+        load_row<T, EPL>(row, a.ne, lane, a.vec, s);
         for (int j = lane; j < a.k; j += 32) {
             const int64_t e = a.ids64 ? static_cast<const int64_t *>(a.ids)[t * a.k + j] : static_cast<const int *>(a.ids)[t * a.k + j];
             if (e >= 0 && e < a.ne) atomicAdd(&hist[e], 1);
         }
         float inv = 1.f;
-        if (as_softmax<EPL>(s, a.softmax)) {
-            softmax_row<EPL>(s, a.ne, lane);
-        } else {
+        if (!a.softmax) {   // past ne x is -inf: 1e-38 each, nothing beside LOW
             float total = 0.f, r;
 #pragma unroll
             for (int i = 0; i < EPL; i++) {
                 sigmoid_pair(s[i], s[i], r);
-                s[i] = expert<EPL>(i, lane) < a.ne ? s[i] : 0.f;
                 total += s[i];
             }
-            inv = 1.f / warp_sum(total);
+            total = warp_sum(total);
+            inv = 1.f / total;
+            if (total < LOW) load_row<T, EPL>(row, a.ne, lane, a.vec, s);
+            if (total < LOW) inv = 0.f;
+        }
+        if (a.softmax || inv == 0.f) {
+            softmax_row<EPL>(s, a.ne, lane);
+            inv = 1.f;
         }
 #pragma unroll
         for (int i = 0; i < EPL; i++) acc[i] = fmaf(s[i], inv, acc[i]);
     }
     if (lane == 0 && rows) atomicAdd(&hist[a.ne], rows);
-    for (int w = 0; w < BAL_WARPS; w++) {   // the warps in order: the same sums every time
-        if (warp == w) {
 #pragma unroll
-            for (int i = 0; i < EPL; i++)
-                if (expert<EPL>(i, lane) < a.ne) sums[expert<EPL>(i, lane)] += acc[i];
-        }
-        __syncthreads();
+    for (int i = 0; i < EPL; i++)
+        if (expert<EPL>(i, lane) < a.ne) sums[warp * a.ne + expert<EPL>(i, lane)] = acc[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.ne; e += W * 32) {   // the warps in order: the same sums every time
+        float p = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; w++) p += sums[w * a.ne + e];
+        a.part_p[(int64_t)blockIdx.x * a.ne + e] = p;
     }
-    for (int e = threadIdx.x; e < a.ne; e += BAL_THREADS) a.part_p[(int64_t)blockIdx.x * a.ne + e] = sums[e];
-    for (int e = threadIdx.x; e <= a.ne; e += BAL_THREADS) a.part_n[(int64_t)blockIdx.x * (a.ne + 1) + e] = hist[e];
+    for (int e = threadIdx.x; e <= a.ne; e += W * 32) a.part_n[(int64_t)blockIdx.x * (a.ne + 1) + e] = hist[e];
 }
 
 // The parts' sums: a cluster of FIN CTAs, each every FIN-th run of 32 experts, 32 rows of parts at a time (one CTA with a
@@ -513,34 +589,51 @@ template <typename T, int EPL> __global__ void __launch_bounds__(THREADS, EPL > 
     float c[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; i++) c[i] = expert<EPL>(i, lane) < a.ne ? a.c[expert<EPL>(i, lane)] : 0.f;
-    for (int64_t t = blockIdx.x * (int64_t)WARPS + (threadIdx.x >> 5); t < a.T; t += (int64_t)gridDim.x * WARPS) {
+    const int64_t step = (int64_t)gridDim.x * WARPS;
+    uint32_t live = ~0u;   // as in balance_kernel
+    int left = 0;
+    for (int64_t t = blockIdx.x * (int64_t)WARPS + (threadIdx.x >> 5); t < a.T; t += step, live >>= 1, left--) {
+        if (a.mask && left == 0) {
+            live = __ballot_sync(0xffffffffu, t + lane * step < a.T && a.mask[t + lane * step]);
+            left = 32;
+        }
         T *out = static_cast<T *>(a.dl) + t * a.ne;
-        float s[EPL];
-        if (a.mask && !a.mask[t]) {
+        const T *row = static_cast<const T *>(a.logits) + t * a.ld;
+        float u[EPL];   // p before its division, times 1 - s
+        if (!(live & 1u)) {
 #pragma unroll
-            for (int i = 0; i < EPL; i++) s[i] = 0.f;
-            store_row<T, EPL>(out, a.ne, lane, a.vec, s);
+            for (int i = 0; i < EPL; i++) u[i] = 0.f;
+            store_row<T, EPL>(out, a.ne, lane, a.vec, u);
             continue;
         }
-        load_row<T, EPL>(static_cast<const T *>(a.logits) + t * a.ld, a.ne, lane, a.vec, s);
-        float r[EPL], total = 0.f, dot = 0.f;
-        const bool soft = as_softmax<EPL>(s, a.softmax);
-        if (soft) softmax_row<EPL>(s, a.ne, lane);
+        load_row<T, EPL>(row, a.ne, lane, a.vec, u);
+        float total = 1.f, dot = 0.f;
+        if (!a.softmax) {
+            total = 0.f;
 #pragma unroll
-        for (int i = 0; i < EPL; i++) {
-            r[i] = 1.f;
-            if (!soft) {
-                sigmoid_pair(s[i], s[i], r[i]);
-                s[i] = expert<EPL>(i, lane) < a.ne ? s[i] : 0.f;
+            for (int i = 0; i < EPL; i++) {
+                float s, r;
+                sigmoid_pair(u[i], s, r);
+                total += s;
+                dot = fmaf(c[i], s, dot);
+                u[i] = s * r;
             }
-            total += s[i];
-            dot = fmaf(c[i], s[i], dot);
+            total = warp_sum(total);
+            if (total < LOW) load_row<T, EPL>(row, a.ne, lane, a.vec, u);
         }
-        const float inv = soft ? 1.f : 1.f / warp_sum(total);
-        dot = warp_sum(dot) * inv;
+        if (a.softmax || total < LOW) {
+            softmax_row<EPL>(u, a.ne, lane);
+            total = 1.f;
+            dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < EPL; i++) s[i] = g * (s[i] * inv) * (c[i] - dot) * r[i];
-        store_row<T, EPL>(out, a.ne, lane, a.vec, s);
+            for (int i = 0; i < EPL; i++) dot = fmaf(c[i], u[i], dot);
+        }
+        const float inv = 1.f / total;
+        dot = warp_sum(dot) * inv;
+        const float f = g * inv;
+#pragma unroll
+        for (int i = 0; i < EPL; i++) u[i] = f * u[i] * (c[i] - dot);
+        store_row<T, EPL>(out, a.ne, lane, a.vec, u);
     }
 }
 
@@ -591,7 +684,8 @@ int qmoe_route(const void *logits, int x_dtype, int64_t ld, const float *bias, i
         topk_group > n_group || (n_group > 1 && n_experts / n_group < 2) || (bias && score == 1))
         return QMOE_ERR_SHAPE;
     DeviceInfo *di;
-    if (int e = current_device(nullptr, &di)) return e;
+    int dev;
+    if (int e = current_device(&dev, &di)) return e;
     rt::Route a{};
     a.logits = logits;
     a.ld = ld;
@@ -609,12 +703,21 @@ int qmoe_route(const void *logits, int x_dtype, int64_t ld, const float *bias, i
     a.counts = counts;
     a.vec = rt::four(logits, x_dtype, ld, n_experts);
     cudaStream_t st = as_stream(stream);
-    const unsigned grid = rt::grid_of(T, *di, 4);
-    if (grid > 1 && cudaMemsetAsync(counts, 0, sizeof(int) * n_experts, st) != cudaSuccess) return QMOE_ERR_LAUNCH;
-    const size_t smem = sizeof(float) * n_experts * (n_group > 1 ? 1 + rt::WARPS : 1);   // at most 36 KB
-    return rt::by_type(x_dtype, n_experts, [&](auto t, auto w) {
-        rt::route_kernel<decltype(t), decltype(w)::value><<<grid, rt::THREADS, smem, st>>>(a);
-        return launch_status();
+    return rt::by_type(x_dtype, n_experts, [&](auto t, auto w) -> int {
+        constexpr int EPL = decltype(w)::value;
+        using X = decltype(t);
+        const int warps = T <= (int64_t)di->sms * 32 ? rt::WARPS : rt::ROUTE_WARPS<EPL>;
+        const int64_t ctas = (T + warps - 1) / warps;
+        const unsigned grid = (unsigned)(ctas < di->sms * (warps == rt::WARPS ? 4 : 1) ? ctas : di->sms * (warps == rt::WARPS ? 4 : 1));
+        const size_t smem = warps * sizeof(rt::Candidates) + sizeof(float) * (EPL * 32 + n_experts * (n_group > 1 ? 1 + warps : 1));
+        auto launch = [&](auto kern, std::atomic<uint64_t> &done) -> int {
+            if (!(done.load(std::memory_order_acquire) >> (dev & 63) & 1) && !ensure_smem(kern, smem, dev, done)) return QMOE_ERR_LAUNCH;
+            if (grid > 1 && cudaMemsetAsync(counts, 0, sizeof(int) * n_experts, st) != cudaSuccess) return QMOE_ERR_LAUNCH;
+            kern<<<grid, warps * 32, smem, st>>>(a);
+            return launch_status();
+        };
+        static std::atomic<uint64_t> done_fast{0}, done_full{0};
+        return a.softmax || a.n_group > 1 ? launch(rt::route_kernel<X, EPL, false>, done_full) : launch(rt::route_kernel<X, EPL, true>, done_fast);
     });
 }
 
@@ -648,7 +751,7 @@ int qmoe_route_backward(const void *logits, int x_dtype, int64_t ld, int64_t T, 
 
 size_t qmoe_balance_workspace_bytes(int64_t T, int n_experts) {
     if (T < 1 || n_experts < 1 || n_experts > rt::MAX_E) return 0;
-    const int64_t parts = (T + rt::BAL_WARPS - 1) / rt::BAL_WARPS;
+    const int64_t parts = (T + 15) / 16;   // at least
     return (size_t)(parts < rt::MAX_PARTS ? parts : rt::MAX_PARTS) * (2 * n_experts + 1) * 4;
 }
 
@@ -660,7 +763,8 @@ int qmoe_balance(const void *logits, int x_dtype, int64_t ld, const void *ids, i
     if (!aligned4(workspace) || (reinterpret_cast<uintptr_t>(ids) & (ids_64 ? 7u : 3u))) return QMOE_ERR_ALIGN;
     if (workspace_bytes < qmoe_balance_workspace_bytes(T, n_experts)) return QMOE_ERR_WORKSPACE;
     DeviceInfo *di;
-    if (int e = current_device(nullptr, &di)) return e;
+    int dev;
+    if (int e = current_device(&dev, &di)) return e;
     rt::Balance a{};
     a.logits = logits;
     a.ld = ld;
@@ -676,15 +780,20 @@ int qmoe_balance(const void *logits, int x_dtype, int64_t ld, const void *ids, i
     a.counts = counts;
     a.c = c;
     a.vec = rt::four(logits, x_dtype, ld, n_experts);
-    int64_t parts = (T + rt::BAL_WARPS - 1) / rt::BAL_WARPS;
-    const int most = 2 * di->sms < rt::MAX_PARTS ? 2 * di->sms : rt::MAX_PARTS;
+    const int warps = n_experts > 512 ? rt::BAL_WARPS<32> : rt::BAL_WARPS<16>;
+    const int64_t parts = (T + warps - 1) / warps;
+    const int most = di->sms < rt::MAX_PARTS ? di->sms : rt::MAX_PARTS;
     a.parts = (int)(parts < most ? parts : most);
     a.part_p = static_cast<float *>(workspace);
     a.part_n = static_cast<int *>(workspace) + (int64_t)a.parts * n_experts;
     cudaStream_t st = as_stream(stream);
     const int rc = rt::by_type(x_dtype, n_experts, [&](auto t, auto w) {
-        rt::balance_kernel<decltype(t), decltype(w)::value>
-            <<<a.parts, rt::BAL_THREADS, sizeof(float) * (2 * n_experts + 1), st>>>(a);
+        static std::atomic<uint64_t> done{0};
+        constexpr int W = rt::BAL_WARPS<decltype(w)::value>;
+        auto kern = rt::balance_kernel<decltype(t), decltype(w)::value>;
+        const size_t smem = sizeof(float) * ((W + 1) * n_experts + 1);   // at most 68 KB
+        if (!(done.load(std::memory_order_acquire) >> (dev & 63) & 1) && !ensure_smem(kern, smem, dev, done)) return QMOE_ERR_LAUNCH;
+        kern<<<a.parts, W * 32, smem, st>>>(a);
         return launch_status();
     });
     if (rc) return rc;
@@ -721,7 +830,7 @@ int qmoe_balance_backward(const void *logits, int x_dtype, int64_t ld, const uin
     a.grad = dloss;
     a.dl = dlogits;
     a.vec = rt::four(logits, x_dtype, ld, n_experts) && rt::four(dlogits, x_dtype, n_experts, n_experts);
-    const unsigned grid = rt::grid_of(T, *di, 8);
+    const unsigned grid = rt::grid_of(T, *di, 4);
     return rt::by_type(x_dtype, n_experts, [&](auto t, auto w) {
         rt::balance_backward_kernel<decltype(t), decltype(w)::value><<<grid, rt::THREADS, 0, as_stream(stream)>>>(a);
         return launch_status();
