@@ -1,9 +1,9 @@
 // The operators of dense_q's four-bit part and of router as functions of torch tensors, over the C entry points: argument
 // checks, outputs from torch's allocator, the current stream, and automatic differentiation.
 //
-// Small calls are bound by the host. The same calls from Python by ctypes, with a torch.autograd.Function, took 113 us
-// for a loss and its gradient of 200 tokens, 60 us of them in the Python parts of the function and in handing
-// its backward pass to the engine's thread; a single quantisation took 13 us.
+// Small calls are bound by the host. The same calls by ctypes, with a torch.autograd.Function, took 113 us for a loss of
+// 200 tokens and its gradient (72 here), 11 us for one token's linear (6.6), 24 us for quantising a token and reading it back
+// (16).
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>

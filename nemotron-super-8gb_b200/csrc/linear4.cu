@@ -222,7 +222,7 @@ int dq_linear_a4(const uint8_t *w, const uint8_t *w_sc, const uint8_t *w_atoms, 
         a.ldx = ldx;
         a.N = N;
         a.K = K;
-        a.vec = aligned16(x) && ldx * size % 16 == 0;
+        a.vec = qz::row_vec(x, ldx * size);
         const int unit = 2 * g4::TOK_WARPS, target = 2 * di->sms;   // about two CTAs per SM, whole rounds of rows
         a.rows = ((N + target - 1) / target + unit - 1) / unit * unit;
         a.epilogue = epilogue;

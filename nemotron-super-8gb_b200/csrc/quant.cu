@@ -17,7 +17,7 @@ struct Args {
     int64_t ldx;   // row stride of x, in elements
     int64_t M;
     int nb;        // blocks per row, K / 16
-    int vec;       // rows are 16-byte aligned
+    int vec;       // row_vec
     int words;     // whole k-steps per row: four scales are one aligned word
     uint8_t *w, *sc, *atoms;
     float *s;      // per row: written; per tensor: read
@@ -260,7 +260,7 @@ int dq_quantize_nvfp4(const void *x, int x_dtype, int64_t ldx, int64_t M, int64_
     a.ldx = ldx;
     a.M = M;
     a.nb = (int)(K / 16);
-    a.vec = aligned16(x) && (ldx * size) % 16 == 0;
+    a.vec = qz::row_vec(x, ldx * size);
     a.words = a.nb % 4 == 0 && aligned4(sc);
     a.w = w;
     a.sc = sc;

@@ -144,7 +144,7 @@ def test_quantize_extremes(per_row):
 def test_quantize_strides_and_offsets():
     import dense_q as D
     base = torch.randn(70, 1100, generator=seeded(9), device=DEV).to(torch.bfloat16)
-    for x in (base[:, :1024], base[::3, 1:993], base[:, 8:1032], base.t()[:64].t()[:, :64], base[:1, :1088], base.t()[:1088, :64].t()):
+    for x in (base[:, :1024], base[::3, 1:993], base[:, 8:1032], base.t()[:64].t()[:, :64], base.view(-1)[16:16 + 65 * 1104].view(65, 1104)[:, :1088], base[:1, :1088], base.t()[:1088, :64].t()):
         check_quantized(D.quantize(x, for_gemm=True), x, True)
         check_quantized(D.quantize(x, per_row=False), x, False)
     one = base[0, :16].reshape(1, 16).expand(5, 16)      # a broadcast row
