@@ -26,6 +26,8 @@ constexpr int MAX_SPLIT = 8;
 
 __device__ int g_status;             // first error of this device's calls since it was last cleared
 
+constexpr int MOST = 64;             // most tokens of a tile of gemm_kernel
+
 template <int TN> struct Plan {   // TN <= 128: a stage holds one atom of token scales per k-step
     static constexpr int B_BYTES = TN * ROWB;
     static constexpr int OFF_B = A_BYTES, OFF_SFA = OFF_B + B_BYTES, OFF_SFB = OFF_SFA + SFA_BYTES;
@@ -34,7 +36,8 @@ template <int TN> struct Plan {   // TN <= 128: a stage holds one atom of token 
     static constexpr int OFF_BAR = STAGES * STAGE;
     static constexpr int NBAR = 2 * STAGES + 5;
     static constexpr int OFF_MISC = OFF_BAR + (NBAR * 8 + 15) / 16 * 16;
-    static constexpr int SMEM = OFF_MISC + 16 + 1024;
+    static constexpr int OFF_COL = OFF_MISC + 16;      // [4][MOST] each epilogue warp's copy of the token scales
+    static constexpr int SMEM = OFF_COL + 4 * MOST * 4 + 1024;
     static_assert(SMEM <= 232448, "fits the 227 KB opt-in");
     // Tensor memory: two accumulators of TN columns and two scale slots.
     static constexpr int SF_COL = 2 * TN;
@@ -97,15 +100,21 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr, int rank) {
     return v;
 }
 
-// 32 tokens' columns of one weight row (a lane): element j at y[at + j * N], for the first `left` of them. Lane j of the
-// warp holds token j's scale in sx.
+// 32 tokens' columns of one weight row (a lane): element j at y[at + j * N], for the first `left` of them, their scales in
+// cs[0 .. 31]. All residuals are loaded before the first store: y might be the same memory, so that between stores each
+// load would wait for memory by itself (2683 x 260 x 768 with a residual: 32 us).
 template <typename T, int EPI>
-__device__ __forceinline__ void store_columns(void *y, const void *res, int64_t at, int64_t N, bool in, int left, const float (&v)[32], float sx, float sw) {
+__device__ __forceinline__ void store_tokens(void *y, const void *res, int64_t at, int64_t N, bool in, int left, const float (&v)[32], float sw, const float *cs) {
+    if (!in) return;
+    T r[32];
+    if (EPI == 2) {
 #pragma unroll
-    for (int j = 0; j < 32; j++) {
-        const float s = __shfl_sync(0xffffffffu, sx, j);
-        if (in && j < left) store_one<T, EPI>(y, res, at + j * N, v[j], s, sw);
+        for (int j = 0; j < 32; j++)
+            if (j < left) r[j] = static_cast<const T *>(res)[at + j * N];
     }
+#pragma unroll
+    for (int j = 0; j < 32; j++)
+        if (j < left) static_cast<T *>(y)[at + j * N] = narrow<T>(finish<T, EPI>(v[j], cs[j], sw, EPI == 2 ? wide(r[j]) : 0.f));
 }
 
 template <int TN, typename T>
@@ -249,6 +258,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                 break;
             }
             const float sw = n < p.N ? p.sw[(int64_t)n * p.sw_step] : 0.f;
+            float *cs = reinterpret_cast<float *>(sm + P::OFF_COL) + warp * MOST;   // a copy per warp: no barrier between warps
+            __syncwarp();
+            for (int c = lane; c < cols; c += 32) cs[c] = p.sx[(int64_t)(m0 + c) * p.sx_step];
+            __syncwarp();
 #pragma unroll 1
             for (int c0 = 0; c0 < TN; c0 += 32) {
                 float v[32];
@@ -260,11 +273,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (lane == 0) mbar_arrive(&acc_free[t & 1]);
                 }
                 if (left <= 0) continue;
-                const float sx = p.sx[(int64_t)(m0 + c0 + min(lane, left - 1)) * p.sx_step];
                 const int64_t at = (int64_t)(m0 + c0) * p.N + n;
-                if (p.epilogue == 0) store_columns<T, 0>(p.y, p.res, at, p.N, n < p.N, left, v, sx, sw);
-                else if (p.epilogue == 1) store_columns<T, 1>(p.y, p.res, at, p.N, n < p.N, left, v, sx, sw);
-                else store_columns<T, 2>(p.y, p.res, at, p.N, n < p.N, left, v, sx, sw);
+                if (p.epilogue == 0) store_tokens<T, 0>(p.y, p.res, at, p.N, n < p.N, left, v, sw, cs + c0);
+                else if (p.epilogue == 1) store_tokens<T, 1>(p.y, p.res, at, p.N, n < p.N, left, v, sw, cs + c0);
+                else store_tokens<T, 2>(p.y, p.res, at, p.N, n < p.N, left, v, sw, cs + c0);
             }
         }
     }
@@ -456,11 +468,17 @@ __device__ __forceinline__ void ld32(const void *p, uint32_t (&v)[8]) {
 template <typename T, int EPI, bool EACH>
 __device__ __forceinline__ void store_run(void *y, const void *res, int64_t at, bool in, int left, const float (&v)[32], float sx, float sw, const float *cs) {
     constexpr int EPV = 32 / sizeof(T);   // elements per store
+    uint32_t rs[32 / EPV][8] = {};
+    if (EPI == 2) {   // all loads before the first store, as in store_tokens
+#pragma unroll
+        for (int u = 0; u < 32 / EPV; u++)
+            if (in && u * EPV < left) ld32(static_cast<const T *>(res) + at + u * EPV, rs[u]);
+    }
 #pragma unroll
     for (int u = 0; u < 32 / EPV; u++) {
         const bool live = in && u * EPV < left;
-        uint32_t r[8] = {}, o[8];
-        if (EPI == 2 && live) ld32(static_cast<const T *>(res) + at + u * EPV, r);
+        const uint32_t(&r)[8] = rs[u];
+        uint32_t o[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             if constexpr (sizeof(T) == 4) {
@@ -476,15 +494,6 @@ __device__ __forceinline__ void store_run(void *y, const void *res, int64_t at, 
         }
         if (live) st32(static_cast<T *>(y) + at + u * EPV, o);
     }
-}
-
-// 32 tokens' columns of one weight row (a lane), their scales in cs.
-template <typename T, int EPI>
-__device__ __forceinline__ void store_tokens(void *y, const void *res, int64_t at, int64_t N, bool in, int left, const float (&v)[32], float sw, const float *cs) {
-    if (!in) return;
-#pragma unroll
-    for (int j = 0; j < 32; j++)
-        if (j < left) store_one<T, EPI>(y, res, at + j * N, v[j], cs[j], sw);
 }
 
 template <int TN, typename T, int EPI>
