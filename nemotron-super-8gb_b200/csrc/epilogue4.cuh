@@ -21,7 +21,8 @@ __device__ __forceinline__ float wide(__half v) { return __half2float(v); }
 template <typename T, int EPI> __device__ __forceinline__ float finish(float v, float sx, float sw, float res) {
     v = __fmul_rn(__fmul_rn(v, sx), sw);
     if (EPI == 1) {
-        const float o = wide(narrow<T>(v)), r = o > 0.f ? o : (o != o ? o : 0.f);
+        float r;
+        asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(wide(narrow<T>(v))));   // relu, NaN kept
         return __fmul_rn(r, r);
     }
     return EPI == 2 ? __fadd_rn(wide(narrow<T>(v)), res) : v;
