@@ -112,15 +112,18 @@ template <typename T> __device__ __forceinline__ uint32_t block16(const Raw<T> &
     asm("{\n\t.reg .b16 t;\n\tcvt.rn.satfinite.e4m3x2.f32 t, %1, %2;\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(sb) : "f"(0.f), "f"(__uint_as_float(m)));
     sb &= 0xFFu;
     if (sb == 0u) return 0u;
-    float f, pre = 1.f;
+    float f;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(e4m3_f32((uint8_t)sb)));
-    if (e >= -116) f *= inv_s;   // one factor for x / (s sc), off by the reciprocal's error alone
-    else pre = inv_s;            // rows of almost nothing: it would overflow
     float q[16];
     widen(v, q);
+    if (e >= -116) {   // one factor for x / (s sc), off by the reciprocal's error alone
+        f *= inv_s;
+    } else {           // rows of almost nothing: it would overflow
+#pragma unroll
+        for (int i = 0; i < 16; i++) q[i] *= inv_s;
+    }
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-        if (e < -116) q[i] *= pre;
         if constexpr (sizeof(T) == 4) q[i] = __uint_as_float(odd13(__float_as_uint(q[i])));
         q[i] = fmaf(q[i], f, 192.f) - 192.f;
     }
