@@ -173,9 +173,9 @@ int qmoe_prefill_grouped(const uint8_t *store, int64_t block_stride, int n_exper
                          void *workspace, size_t workspace_bytes, void *stream);
 
 /* No counterpart in the reference. Bound, in SM clock cycles, on each device-side wait of the kernels that wait
- * (the pipeline roles of qmoe_prefill_grouped's tensor-core GEMMs) on the current device, from the next call on;
+ * (the pipeline roles of qmoe_prefill_grouped's and dq_gemm_nvfp4's tensor-core GEMMs) on the current device, from the next call on;
  * cycles <= 0 restores the default of 4e9 cycles (about 2 s). A wait that runs out records QMOE_ERR_TIMEOUT in the
- * workspace status word and the kernel stops: every copy it started lands and every MMA it issued completes
+ * workspace status word (dq_gemm_nvfp4: the device's, dq_gemm_nvfp4_status) and the kernel stops: every copy it started lands and every MMA it issued completes
  * (each waited for with the default bound) before it frees its tensor memory and returns; its outputs are then
  * undefined and the next call runs normally. Meant for failure handling and its tests: a short bound makes
  * ordinary calls time out. */
@@ -200,7 +200,7 @@ int qmoe_route_decode(const float *logits, const float *bias, int n_experts, int
  * groups with the largest sums of their two best choices keep them, the others' are 0 (softmax: -inf). ids [T, top_k]
  * the largest choices in decreasing order, ties to the lower id, a NaN last; weights [T, top_k] = score, / (their sum +
  * 1e-20) when norm != 0, * scaling; counts [n_experts]: tokens that chose each expert. n_experts <= 1024, top_k <= 32,
- * n_group <= 32 groups of at least two. */
+ * n_group <= 32 groups of at least two, of a softmax the kept ones with at least top_k experts. */
 int qmoe_route(const void *logits, int x_dtype, int64_t ld, const float *bias, int64_t T, int n_experts, int top_k,
                int n_group, int topk_group, int norm, int score, float scaling, int64_t *ids, float *weights,
                int32_t *counts, void *stream);
@@ -322,8 +322,8 @@ int dq_dequant_nvfp4(const uint8_t *w, const uint8_t *sc, const float *s, int s_
  * weights w [N, K/2], both scales as atoms, accumulated in fp32; sw, sx one value or one per row. y [M, N] in y_dtype,
  * rounded once and then as dq_gemv_nvfp4_bf16's epilogues: 0 the product, 1 relu^2 of it, 2 the sum with residual
  * [M, N] (of y_dtype). Block scales are non-negative (the sign bit is not read). Any M, N >= 1; K a multiple of 32;
- * codes and atoms 16-byte aligned. Sums run in a fixed
- * order: the same call gives the same bits. A device-side wait that runs out (qmoe_set_wait_cycles) records QMOE_ERR_TIMEOUT, read by dq_gemm_nvfp4_status. */
+ * codes and atoms 16-byte aligned. Sums run in a fixed order: the same call gives the same bits. A device-side wait
+ * that runs out (its limit is qmoe_set_wait_cycles') records QMOE_ERR_TIMEOUT, read by dq_gemm_nvfp4_status. */
 int dq_gemm_nvfp4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int sw_per_row, const uint8_t *x,
                   const uint8_t *x_atoms, const float *sx, int sx_per_row, int M, int N, int K, int epilogue,
                   const void *residual, void *y, int y_dtype, void *stream);

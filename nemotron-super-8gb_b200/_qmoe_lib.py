@@ -100,7 +100,7 @@ def bind():
         spec = importlib.util.spec_from_file_location("qmoe_torch", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        mod.set_error_class(QmoeError)
+        mod.set_error_classes(QmoeError, torch.OutOfMemoryError)
         _bind = mod
     return _bind
 

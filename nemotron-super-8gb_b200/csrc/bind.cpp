@@ -88,13 +88,23 @@ void check_tensors(const Tensor &w, const Tensor &sc, const Tensor &s, bool per_
                 name, " must be contiguous uint8 [", N, ", ", width, "]");
     REQUIRE(s.scalar_type() == at::kFloat && s.numel() == (per_row ? N : 1) && s.is_contiguous(),
             "s must be float32, one value (nvfp4) or one per row (nvfp4_rows)");
+}
+void check_device(const Tensor &w, const Tensor &sc, const Tensor &s) {
     REQUIRE(w.is_cuda() && sc.device() == w.device() && s.device() == w.device(), "libqmoe_b200 works on CUDA tensors only, all of a weight on one device");
 }
 
 int64_t atoms_bytes(int64_t rows, int64_t K) { return (rows + 127) / 128 * ((K + 63) / 64) * 512; }
 
+// A quantised matrix as a product's operand: its tensors, and its scale atoms where it has them.
+void check_operand(const Tensor &w, const Tensor &sc, const OptTensor &atoms, const Tensor &s, bool per_row, int64_t N, int64_t K) {
+    check_tensors(w, sc, s, per_row, N, K);
+    REQUIRE(!atoms || (atoms->scalar_type() == at::kByte && atoms->numel() == atoms_bytes(N, K) && atoms->is_contiguous() && atoms->device() == w.device()),
+            "sca must be the ", atoms_bytes(N, K), " bytes that prepare makes of this weight's scales, on its device");
+}
+
 Tensor scale_atoms(const Tensor &w, const Tensor &sc, const Tensor &s, bool per_row, int64_t N, int64_t K) {
     check_tensors(w, sc, s, per_row, N, K);
+    check_device(w, sc, s);
     const c10::cuda::CUDAGuard guard(sc.device());
     const Tensor atoms = empty({atoms_bytes(N, K)}, sc, at::kByte);
     if (N) status(dq_scale_atoms(data<uint8_t>(sc), N, K, data<uint8_t>(atoms), stream_of(sc)), "dq_scale_atoms");
@@ -153,7 +163,10 @@ Tensor gemm(const Tensor &w, const Tensor &wsc, OptTensor watoms, const Tensor &
     REQUIRE(dtype_code(dtype) >= 0, "unsupported output dtype ", dtype);
     check_weight(w, N, Kw, K, x.device());
     const int ep = epilogue(act, residual, M, N, dtype, x.device());
-    REQUIRE(x.is_cuda(), "libqmoe_b200 works on CUDA tensors only (got a CPU tensor)");
+    check_operand(w, wsc, watoms, ws, w_rows, N, K);
+    check_operand(x, xsc, xatoms, xs, x_rows, M, K);
+    check_device(w, wsc, ws);
+    check_device(x, xsc, xs);
     REQUIRE(M <= (1 << 24), "gemm: at most 2^24 rows");
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor y = empty({M, N}, x, dtype);
@@ -176,11 +189,16 @@ Tensor linear_a4(const Tensor &w, const Tensor &sc, OptTensor atoms, const Tenso
     const Tensor x = rows_of(x0.dim() == 2 ? x0 : x0.reshape({K ? x0.numel() / K : 0, K}), ld);
     const int64_t M = x.size(0);
     check_weight(w, N, Kw, K, x.device());
-    if (residual) residual = residual->reshape({-1, N});
-    const int ep = epilogue(act, residual, M, N, x.scalar_type(), x.device());
-    const c10::cuda::CUDAGuard guard(x.device());
+    check_operand(w, sc, atoms, s, w_rows, N, K);
+    check_device(w, sc, s);
     std::vector<int64_t> shape = x0.sizes().vec();
     shape.back() = N;
+    if (residual) {
+        REQUIRE(residual->sizes() == shape, "gemm: the residual has the output's shape ", at::IntArrayRef(shape), " (got ", residual->sizes(), ")");
+        residual = residual->reshape({M, N});
+    }
+    const int ep = epilogue(act, residual, M, N, x.scalar_type(), x.device());
+    const c10::cuda::CUDAGuard guard(x.device());
     const Tensor y = empty(shape, x, x.scalar_type());
     if (M && N) {
         REQUIRE(M <= (1 << 24), "gemm: at most 2^24 rows");
@@ -267,6 +285,7 @@ py::tuple route(const Tensor &logits, OptTensor bias, int64_t top_k, double scal
     REQUIRE(top_k >= 1 && top_k <= std::min<int64_t>(32, E), "top_k must lie in 1..", std::min<int64_t>(32, E), " (got ", top_k, ")");
     REQUIRE(n_group >= 1 && n_group <= 32 && E % n_group == 0 && topk_group >= 1 && topk_group <= n_group && (n_group == 1 || E / n_group >= 2),
             E, " experts do not split into ", n_group, " groups of two or more, ", topk_group, " of them kept");
+    REQUIRE(sc == 0 || top_k <= E / n_group * topk_group, "a softmax router leaves ", E / n_group * topk_group, " experts in ", topk_group, " groups, top_k is ", top_k);
     if (bias) {
         REQUIRE(sc == 0, "a softmax router takes no bias");
         REQUIRE(bias->dim() == 1 && bias->size(0) == E && bias->device() == logits.device(), "bias must be [E], on the logits' device");
@@ -334,6 +353,7 @@ py::tuple balance_loss(const Tensor &logits, const Tensor &ids0, OptTensor mask,
     REQUIRE(ids0.dim() == 2 && ids0.size(0) == T && ids0.size(1) >= 1 && (ids0.scalar_type() == at::kLong || ids0.scalar_type() == at::kInt),
             "ids must be int64 or int32 [T, k] with k >= 1");
     REQUIRE(ids0.device() == logits.device(), "ids must be on the logits' device");
+    REQUIRE(T * ids0.size(1) <= INT32_MAX, "counts are int32: at most 2^31 - 1 ids (got ", T * ids0.size(1), ")");
     const Tensor ids = ids0.contiguous();
     if (mask) {
         REQUIRE(mask->dim() == 1 && mask->size(0) == T && mask->scalar_type() == at::kBool && mask->device() == logits.device(),
@@ -348,17 +368,19 @@ py::tuple balance_loss(const Tensor &logits, const Tensor &ids0, OptTensor mask,
     return py::make_tuple(loss, n);
 }
 
-py::object error_class;
+py::object error_class, memory_class;
 
 } // namespace
 
 PYBIND11_MODULE(qmoe_torch, m) {
-    m.def("set_error_class", [](py::object c) { error_class = std::move(c); });
+    m.def("set_error_classes", [](py::object c, py::object m) { error_class = std::move(c), memory_class = std::move(m); });
     py::register_exception_translator([](std::exception_ptr p) {
         try {
             if (p) std::rethrow_exception(p);
         } catch (const Refused &e) {
             PyErr_SetString(error_class ? error_class.ptr() : PyExc_RuntimeError, e.what());
+        } catch (const c10::OutOfMemoryError &e) {
+            PyErr_SetString(memory_class ? memory_class.ptr() : PyExc_MemoryError, e.what_without_backtrace());
         }
     });
     m.def("quantize", &quantize);
@@ -368,5 +390,5 @@ PYBIND11_MODULE(qmoe_torch, m) {
     m.def("linear_a4", &linear_a4);
     m.def("route", &route);
     m.def("balance_loss", &balance_loss);
-    m.add_object("_cleanup", py::capsule([] { error_class = py::object(); }));
+    m.add_object("_cleanup", py::capsule([] { error_class = memory_class = py::object(); }));
 }

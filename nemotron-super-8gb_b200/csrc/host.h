@@ -70,6 +70,7 @@ inline int launch_status() {
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 inline bool valid_dtype(int dt) { return dt == QMOE_DT_F32 || dt == QMOE_DT_BF16 || dt == QMOE_DT_F16; }

@@ -291,7 +291,7 @@ int dq_dequant_nvfp4(const uint8_t *w, const uint8_t *sc, const float *s, int s_
     if (!w || !sc || !s || !out) return QMOE_ERR_NULL;
     if (K < 16 || (K % 16) || K > (1 << 24) || r0 < 0 || r1 < r0 || r1 > N) return QMOE_ERR_SHAPE;
     if (!valid_dtype(out_dtype)) return QMOE_ERR_DTYPE;
-    if (reinterpret_cast<uintptr_t>(w) & 7u) return QMOE_ERR_ALIGN;
+    if ((reinterpret_cast<uintptr_t>(w) & 7u) || !aligned4(s) || reinterpret_cast<uintptr_t>(out) % (out_dtype == QMOE_DT_F32 ? 4 : 2)) return QMOE_ERR_ALIGN;
     if (int e = current_device(nullptr, nullptr)) return e;
     if (r1 == r0) return QMOE_OK;
     const int nb = (int)(K / 16), vec = aligned16(out);

@@ -165,7 +165,7 @@ __device__ __forceinline__ void keep_groups(float (&c)[EPL], const Route &a, flo
             b2 = fmaxf(fmaxf(b2, o2), fminf(b1, o1));
             b1 = fmaxf(b1, o1);
         }
-        if (lane == g) mine = b1 + b2;
+        if (lane == g) mine = fmaxf(b1 + b2, -INFINITY);   // of opposite infinities: last
     }
     int rank = 0;
     for (int g = 0; g < a.n_group; g++) {
@@ -320,7 +320,8 @@ __device__ __forceinline__ void choose(const Route &a, int64_t t, int lane, cons
 }
 
 // blockDim.x / 32 tokens at a time, up to ROUTE_WARPS. Every CTA adds its counts to the global ones at its end, so many
-// tokens take one large CTA per SM (16384 x 512: 29 us with four of eight warps), few tokens small ones on many SMs.
+// tokens take one large CTA per SM, up to 20 tokens per SM small CTAs of WARPS, up to four per SM (T x 512, small against
+// large: 1184 tokens 8.3 and 10.4 us, 2960 12.2 and 12.4, 4736 14.4 and 11.8, 37888 47 and 42).
 template <int EPL> constexpr int ROUTE_WARPS = EPL > 16 ? 16 : 32;
 template <typename T, int EPL, bool FAST> __global__ void __launch_bounds__(ROUTE_WARPS<EPL> * 32) route_kernel(const Route a) {
     constexpr int SLOTS = EPL * 32;
@@ -382,8 +383,10 @@ template <typename T, int EPL> __global__ void __launch_bounds__(THREADS) route_
     __syncwarp();
     for (int64_t t = blockIdx.x * (int64_t)WARPS + (threadIdx.x >> 5); t < a.T; t += (int64_t)gridDim.x * WARPS) {
         const T *x = static_cast<const T *>(a.logits) + t * a.ld;
-        const int id = lane < a.k ? (int)a.ids[t * a.k + lane] : 0;
-        float ds = lane < a.k ? a.dw[t * a.k + lane] * a.scaling : 0.f;
+        const int64_t id64 = lane < a.k ? a.ids[t * a.k + lane] : -1;
+        const bool on = id64 >= 0 && id64 < a.ne;   // an id that route cannot have given takes no part
+        const int id = on ? (int)id64 : 0;
+        float ds = on ? a.dw[t * a.k + lane] * a.scaling : 0.f;
         float p[EPL];
         float s = 0.f;
         if (a.softmax) {
@@ -393,19 +396,19 @@ template <typename T, int EPL> __global__ void __launch_bounds__(THREADS) route_
             for (int i = 0; i < EPL; i++)
                 if (expert<EPL>(i, lane) < a.ne) row[expert<EPL>(i, lane)] = p[i];
             __syncwarp();
-            if (lane < a.k) s = row[id];
+            if (on) s = row[id];
             __syncwarp();
             for (int e = lane; e < a.ne; e += 32) row[e] = 0.f;
             __syncwarp();
-        } else if (lane < a.k) {
+        } else if (on) {
             s = sigmoid(wide(x[id]));
         }
         if (a.norm) {
             const float total = warp_sum(s) + 1e-20f;
             ds = (ds - warp_sum(ds * s) / total) / total;
         }
-        const float dot = a.softmax ? warp_sum(lane < a.k ? ds * s : 0.f) : 0.f;
-        if (lane < a.k) row[id] = a.softmax ? ds : ds * s * (1.f - s);
+        const float dot = a.softmax ? warp_sum(on ? ds * s : 0.f) : 0.f;
+        if (on) row[id] = a.softmax ? ds : ds * s * (1.f - s);
         __syncwarp();
         float d[EPL];
 #pragma unroll
@@ -416,7 +419,7 @@ template <typename T, int EPL> __global__ void __launch_bounds__(THREADS) route_
         }
         store_row<T, EPL>(static_cast<T *>(a.dl) + t * a.ne, a.ne, lane, a.vec, d);
         __syncwarp();
-        if (lane < a.k) row[id] = 0.f;
+        if (on) row[id] = 0.f;
         __syncwarp();
     }
 }
@@ -663,11 +666,13 @@ static unsigned grid_of(int64_t T, const DeviceInfo &di, int per_sm) {
     return (unsigned)(g < most ? g : most);
 }
 
+static bool aligned(const void *p, int dt) { return reinterpret_cast<uintptr_t>(p) % (dt == QMOE_DT_F32 ? 4 : 2) == 0; }
+
 static int check_logits(const void *logits, int dt, int64_t ld, int64_t T, int ne, int k, int score) {
     if (!logits) return QMOE_ERR_NULL;
     if (T < 1 || T > 0x7FFFFFFF || ne < 1 || ne > MAX_E || k < 1 || ld < ne || score < 0 || score > 1) return QMOE_ERR_SHAPE;
     if (!valid_dtype(dt)) return QMOE_ERR_DTYPE;
-    return reinterpret_cast<uintptr_t>(logits) % (dt == QMOE_DT_F32 ? 4 : 2) ? QMOE_ERR_ALIGN : QMOE_OK;
+    return aligned(logits, dt) ? QMOE_OK : QMOE_ERR_ALIGN;
 }
 
 } // namespace rt
@@ -683,8 +688,10 @@ int qmoe_route(const void *logits, int x_dtype, int64_t ld, const float *bias, i
     if (!ids || !weights || !counts) return QMOE_ERR_NULL;
     if (int e = rt::check_logits(logits, x_dtype, ld, T, n_experts, top_k, score)) return e;
     if (top_k > rt::MAX_K || top_k > n_experts || n_group < 1 || n_group > 32 || n_experts % n_group || topk_group < 1 ||
-        topk_group > n_group || (n_group > 1 && n_experts / n_group < 2) || (bias && score == 1))
+        topk_group > n_group || (n_group > 1 && n_experts / n_group < 2) || (bias && score == 1) ||
+        (score == 1 && top_k > n_experts / n_group * topk_group))
         return QMOE_ERR_SHAPE;
+    if (!aligned4(bias) || !aligned8(ids) || !aligned4(weights) || !aligned4(counts)) return QMOE_ERR_ALIGN;
     DeviceInfo *di;
     int dev;
     if (int e = current_device(&dev, &di)) return e;
@@ -708,7 +715,7 @@ int qmoe_route(const void *logits, int x_dtype, int64_t ld, const float *bias, i
     return rt::by_type(x_dtype, n_experts, [&](auto t, auto w) -> int {
         constexpr int EPL = decltype(w)::value;
         using X = decltype(t);
-        const int warps = T <= (int64_t)di->sms * 32 ? rt::WARPS : rt::ROUTE_WARPS<EPL>;
+        const int warps = T <= (int64_t)di->sms * 20 ? rt::WARPS : rt::ROUTE_WARPS<EPL>;
         const int64_t ctas = (T + warps - 1) / warps;
         const unsigned grid = (unsigned)(ctas < di->sms * (warps == rt::WARPS ? 4 : 1) ? ctas : di->sms * (warps == rt::WARPS ? 4 : 1));
         const size_t smem = warps * sizeof(rt::Candidates) + sizeof(float) * (EPL * 32 + n_experts * (n_group > 1 ? 1 + warps : 1));
@@ -728,6 +735,7 @@ int qmoe_route_backward(const void *logits, int x_dtype, int64_t ld, int64_t T, 
     if (!ids || !dweights || !dlogits) return QMOE_ERR_NULL;
     if (int e = rt::check_logits(logits, x_dtype, ld, T, n_experts, top_k, score)) return e;
     if (top_k > rt::MAX_K || top_k > n_experts) return QMOE_ERR_SHAPE;
+    if (!aligned8(ids) || !aligned4(dweights) || !rt::aligned(dlogits, x_dtype)) return QMOE_ERR_ALIGN;
     DeviceInfo *di;
     if (int e = current_device(nullptr, &di)) return e;
     rt::Route a{};
@@ -762,7 +770,8 @@ int qmoe_balance(const void *logits, int x_dtype, int64_t ld, const void *ids, i
                  size_t workspace_bytes, void *stream) {
     if (!ids || !loss || !counts || !c || !workspace) return QMOE_ERR_NULL;
     if (int e = rt::check_logits(logits, x_dtype, ld, T, n_experts, top_k, score)) return e;
-    if (!aligned4(workspace) || (reinterpret_cast<uintptr_t>(ids) & (ids_64 ? 7u : 3u))) return QMOE_ERR_ALIGN;
+    if (T * top_k > INT32_MAX) return QMOE_ERR_SHAPE;   // counts are 32 bits
+    if (!aligned4(workspace) || !(ids_64 ? aligned8(ids) : aligned4(ids)) || !aligned4(loss) || !aligned4(counts) || !aligned4(c)) return QMOE_ERR_ALIGN;
     if (workspace_bytes < qmoe_balance_workspace_bytes(T, n_experts)) return QMOE_ERR_WORKSPACE;
     DeviceInfo *di;
     int dev;
@@ -819,6 +828,7 @@ int qmoe_balance_backward(const void *logits, int x_dtype, int64_t ld, const uin
                           int score, const float *c, const float *dloss, void *dlogits, void *stream) {
     if (!c || !dloss || !dlogits) return QMOE_ERR_NULL;
     if (int e = rt::check_logits(logits, x_dtype, ld, T, n_experts, 1, score)) return e;
+    if (!aligned4(c) || !aligned4(dloss) || !rt::aligned(dlogits, x_dtype)) return QMOE_ERR_ALIGN;
     DeviceInfo *di;
     if (int e = current_device(nullptr, &di)) return e;
     rt::Balance a{};

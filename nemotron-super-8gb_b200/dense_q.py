@@ -144,8 +144,9 @@ def quantize(x, per_row=True, for_gemm=False):
     """x [M, K] (bf16, fp16 or fp32; K a multiple of 16; rows may be strided) -> quantized dict: codes "w" [M, K/2],
     block scales "sc" [M, K/16] (e4m3 bytes), "s" f32 [M] with fmt "nvfp4_rows" (per_row), or [1] with fmt "nvfp4"
     (one scale for the tensor: a weight of this module); with for_gemm also "sca", the scales as gemm reads them (what
-    prepare adds, in the same pass). s is the smallest power of two with amax <= 2688 s, scales and codes the nearest, ties to even. A 16-element block that holds an
-    infinity or a NaN reads back as NaN; the others are as if that value were zero."""
+    prepare adds, in the same pass). s is the smallest power of two with amax <= 2688 s, scales and codes the nearest,
+    ties to even. A 16-element block that holds an infinity or a NaN reads back as NaN; the others are as if that value
+    were zero."""
     w, sc, s, sca = C.bind().quantize(x, per_row, for_gemm)
     q = {"fmt": "nvfp4_rows" if per_row else "nvfp4", "w": w, "sc": sc, "s": s, "N": x.shape[0], "K": x.shape[1]}
     if for_gemm:
@@ -168,10 +169,10 @@ def prepare(q):
 
 
 def gemm(q, xq, dtype=torch.bfloat16, act=None, residual=None):
-    """y [M, N] in dtype = dequant(xq) @ dequant(q).T for two NVFP4 dicts (xq of quantize: activations; q: a weight,
-    either without "sca" has its scales laid out in this call), products exact, fp32 sums in a
-    fixed order. act "relu2": relu(y)^2; residual [M, N] in dtype: y + residual; each on y rounded to dtype, as the
-    unfused torch operators. K a multiple of 32."""
+    """y [M, N] in dtype = dequant(xq) @ dequant(q).T for two NVFP4 dicts (xq of quantize: activations; q: a weight;
+    either without "sca" has its scales laid out in this call), products exact, fp32 sums in a fixed order. act "relu2":
+    relu(y)^2; residual [M, N] in dtype: y + residual; each on y rounded to dtype, as the unfused torch operators. K a
+    multiple of 32."""
     _nvfp4(q)
     _nvfp4(xq)
     return C.bind().gemm(q["w"], q["sc"], q.get("sca"), q["s"], q["fmt"] == "nvfp4_rows", q["N"], q["K"], xq["w"], xq["sc"],

@@ -197,9 +197,9 @@ def prefill_status(device=None, clear=True):
 
 
 def set_wait_cycles(cycles, device=None):
-    """Bound, in SM clock cycles, on each device-side wait of moe_prefill's GEMM pipelines on the device (the
+    """Bound, in SM clock cycles, on each device-side wait of moe_prefill's and dense_q.gemm's pipelines on the device (the
     current one by default), from the next call on; cycles <= 0 restores the default (4e9, about 2 s). A wait
-    that runs out records QMOE_ERR_TIMEOUT (prefill_status() == 4) and the kernel stops after its copies and
+    that runs out records QMOE_ERR_TIMEOUT (prefill_status() or gemm_status() == 4) and the kernel stops after its copies and
     MMAs in flight complete. No counterpart in the reference."""
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
         C.call("qmoe_set_wait_cycles", int(cycles))

@@ -13,8 +13,8 @@ def route(logits, bias=None, top_k=22, scaling=5.0, n_group=1, topk_group=1, nor
     Score sigmoid(logit), choice score + bias [E] f32; with n_group > 1 only the topk_group groups whose two best
     choices have the largest sum keep theirs (the others' become 0, as the model's router has it); the top_k <= 32
     largest choices; weight = score, divided by the sum of the chosen (+ 1e-20) with norm_topk_prob, times scaling.
-    score "softmax": the softmax over the experts, chosen by the logits, no bias, groups left out entirely. A NaN is
-    chosen last. Differentiable in the logits through the weights."""
+    score "softmax": the softmax over the experts, chosen by the logits, no bias, groups left out entirely (the kept
+    ones need top_k experts). A NaN is chosen last. Differentiable in the logits through the weights."""
     return C.bind().route(logits, bias, top_k, scaling, n_group, topk_group, norm_topk_prob, score)
 
 
@@ -22,6 +22,6 @@ def balance_loss(logits, ids, mask=None, score="sigmoid", coef=1.0):
     """logits [T, E] (fp32, bf16 or fp16), ids [T, k] int64 or int32 (of route) -> (loss f32 [], counts int32 [E]):
     loss = coef * sum_e f_e P_e with f_e = E * counts_e / (k * T') and P_e the mean over tokens of score_e / sum of the
     token's scores; 1 * coef when the experts are evenly loaded. mask [T] bool: tokens with False (padding) count
-    nowhere, T' are the others; none left: loss 0. Ids outside [0, E) are not counted. Differentiable in the logits
+    nowhere, T' are the others; none left: loss 0. Ids outside [0, E) are not counted, one that is twice in a row counts twice. Differentiable in the logits
     (f is held fixed, as the counts have no gradient). Sums run in a fixed order."""
     return C.bind().balance_loss(logits, ids, mask, score, coef)

@@ -92,6 +92,28 @@ def test_python_refusals():
         D.gemm(rows, rows, dtype=torch.float64)
 
 
+def test_an_operand_is_looked_at_in_every_call():
+    """A dict whose tensors no longer belong together is refused, with its laid-out scales too: the kernels trust sizes."""
+    import _qmoe_lib as C
+    import dense_q as D
+    q = {"fmt": "nvfp4", "w": torch.zeros(4, 32, dtype=torch.uint8), "sc": torch.zeros(4, 4, dtype=torch.uint8), "s": torch.ones(1),
+         "sca": torch.zeros(512, dtype=torch.uint8), "N": 4, "K": 64}
+    for bad, word in (({"w": q["w"][:3]}, "w must"), ({"w": torch.zeros(4, 64, dtype=torch.uint8)[:, ::2]}, "w must"),
+                      ({"sc": q["sc"][:3]}, "sc must"), ({"s": torch.ones(2)}, "s must"), ({"sca": q["sca"][:256]}, "sca must"),
+                      ({"sca": torch.zeros(512)}, "sca must"), ({"N": 129}, "w must")):
+        with pytest.raises(C.QmoeError, match=word):
+            D.gemm({**q, **bad}, q)
+        with pytest.raises(C.QmoeError, match=word):
+            D.gemm(q, {**q, **bad})
+
+
+def test_dequant_alignment(lib):
+    a = P(256)
+    assert lib.dq_dequant_nvfp4(a, a, P(258), 1, 4, 64, 0, 4, a, 1, None) == 2
+    assert lib.dq_dequant_nvfp4(a, a, a, 1, 4, 64, 0, 4, P(257), 1, None) == 2
+    assert lib.dq_dequant_nvfp4(a, a, a, 1, 4, 64, 0, 4, P(258), 0, None) == 2
+
+
 def test_linear_arguments(lib):
     a = P(256)
     need = lib.dq_linear_a4_workspace_bytes(5, 64)

@@ -323,3 +323,46 @@ def test_linear_of_few_tokens(M, N, K):
         x[0, 5] = float("nan")
         y = D.qlinear_a4(q, x)
         assert torch.isnan(y[0]).all() and torch.isfinite(y[1:]).all() and (M == 1 or not y[M - 1].any())
+
+
+def test_residual_of_another_shape_is_refused():
+    import _qmoe_lib as C
+    import dense_q as D
+    q = D.prepare(D.quantize(torch.ones(6, 64, device=DEV), False))
+    x = torch.ones(2, 3, 64, device=DEV)
+    D.qlinear_a4(q, x, residual=torch.ones(2, 3, 6, device=DEV))
+    for shape in ((6, 6), (3, 2, 6), (1, 1, 6), (2, 3, 5)):
+        with pytest.raises(C.QmoeError, match="residual"):
+            D.qlinear_a4(q, x, residual=torch.ones(shape, device=DEV))
+    with pytest.raises(C.QmoeError, match="residual"):
+        D.qlinear_a4(q, x, residual=torch.ones(2, 3, 6, device=DEV, dtype=torch.float16))
+    rows = {**q, "N": 5}
+    with pytest.raises(C.QmoeError, match="w must"):
+        D.qlinear_a4(rows, x)
+
+
+def test_no_memory_is_torchs_own_error():
+    import dense_q as D
+    x = torch.zeros(1, 4096, device=DEV).expand(1 << 28, 4096)    # a copy would take 4 TB
+    with pytest.raises(torch.OutOfMemoryError):
+        D.quantize(x)
+    assert torch.equal(D.quantize(x[:3])["s"], torch.full((3,), 2.0 ** -126, device=DEV))
+
+
+def test_two_streams_at_once():
+    """Calls of every form in flight on two streams: the same bits as one after the other."""
+    import dense_q as D
+    g = seeded(91)
+    q = D.prepare(D.quantize(torch.randn(1000, 2048, generator=g, device=DEV), False))
+    xs = [torch.randn(M, 2048, generator=g, device=DEV).to(torch.bfloat16) for M in (1, 3, 30, 60, 300, 700)]
+    want = [D.qlinear_a4(q, x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got += [(j, D.qlinear_a4(q, xs[j])) for j in (range(len(xs)) if i else reversed(range(len(xs))))]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[j]) for j, y in got) and D.gemm_status() == 0

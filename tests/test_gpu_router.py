@@ -374,3 +374,83 @@ def test_only_what_is_asked_for_is_differentiated():
     bias = torch.zeros(16, device=DEV, requires_grad=True)
     R.route(x, bias, top_k=2)[1].sum().backward()
     assert bias.grad is None
+
+
+def test_groups_of_opposite_infinities():
+    """A group whose two best choices are +inf and -inf has no sum: it comes last, and topk_group groups are kept."""
+    import router as R
+    bias = torch.zeros(8, device=DEV)
+    bias[0], bias[1] = float("inf"), -float("inf")
+    ids, _, _ = R.route(torch.zeros(3, 8, device=DEV), bias, top_k=8, n_group=4, topk_group=2)
+    # groups 1 and 2 are kept with choices of 0.5, the others' become 0: ties to the lower id
+    assert ids.tolist() == [[2, 3, 4, 5, 0, 1, 6, 7]] * 3
+
+
+def test_ids_that_are_none_take_no_part_in_the_gradient():
+    """The C entry with ids outside the experts (a caller's own list): as if they were not chosen."""
+    import _qmoe_lib as C
+    g = seeded(71)
+    x = torch.randn(5, 40, generator=g, device=DEV)
+    dw = torch.randn(5, 6, generator=g, device=DEV)
+    ids = torch.topk(x, 6)[1]
+    ids[:, 2] = torch.tensor([-1, 40, 1 << 40, -(1 << 40), 41], device=DEV)
+    for score in (0, 1):
+        for norm in (0, 1):
+            dl = torch.empty_like(x)
+            C.call("qmoe_route_backward", C.ptr(x), 0, 40, 5, 40, 6, norm, score, 5.0, C.ptr(ids), C.ptr(dw), C.ptr(dl), C.stream_of(x))
+            y = x.double().requires_grad_()
+            keep = [0, 1, 3, 4, 5]
+            w = weights64(y, ids[:, keep], 5.0, norm == 1, ("sigmoid", "softmax")[score])
+            ref = torch.autograd.grad(w, y, dw[:, keep].double())[0]
+            assert bool(((dl.double() - ref).abs() <= TOL * 5 * dw.abs().double().sum(-1, keepdim=True)).all())
+
+
+def test_route_refusals():
+    import _qmoe_lib as C
+    import router as R
+    x = torch.zeros(4, 64, device=DEV)
+    ids = torch.zeros(4, 2, dtype=torch.int64, device=DEV)
+    for bad, word in ((lambda: R.route(x, score="softmax", top_k=17, n_group=8, topk_group=2), "leaves 16"),
+                      (lambda: R.route(x, torch.zeros(64, device=DEV), score="softmax"), "no bias"),
+                      (lambda: R.route(x, torch.zeros(63, device=DEV)), "bias must"), (lambda: R.route(x, top_k=33), "top_k"),
+                      (lambda: R.route(x, n_group=5), "groups"), (lambda: R.balance_loss(x, ids[:3]), "ids must"),
+                      (lambda: R.balance_loss(x, ids.float()), "ids must"), (lambda: R.balance_loss(x, ids.cpu()), "device"),
+                      (lambda: R.balance_loss(x, ids, torch.ones(4, device=DEV)), "mask must")):
+        with pytest.raises(C.QmoeError, match=word):
+            bad()
+
+
+@pytest.mark.parametrize("T", [1, 7, 8, 9, 2959, 2960, 2961, 3500, 4737])
+def test_route_counts_at_the_launch_borders(T):
+    check_route(torch.randn(T, 96, generator=seeded(T), device=DEV), None, 6, grad=False)
+
+
+def test_backward_into_a_graph():
+    """loss.backward() captured after warm-up, both operators together, twice through a non-leaf; replayed on new inputs."""
+    import router as R
+    x = torch.randn(300, 64, generator=seeded(81), device=DEV, requires_grad=True)
+    gate = torch.randn(128, 64, generator=seeded(82), device=DEV, requires_grad=True)
+
+    def step():
+        ids, w, _ = R.route(x @ gate.t(), None, top_k=4, norm_topk_prob=True)
+        (R.balance_loss(x @ gate.t(), ids, coef=0.1)[0] + w.square().sum()).backward()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    x.grad.zero_(), gate.grad.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for seed in (83, 84):
+        with torch.no_grad():
+            x.copy_(torch.randn(300, 64, generator=seeded(seed), device=DEV))
+        x.grad.zero_(), gate.grad.zero_()
+        graph.replay()
+        got = x.grad.clone(), gate.grad.clone()
+        x.grad.zero_(), gate.grad.zero_()
+        step()
+        for a, b in zip(got, (x.grad, gate.grad)):
+            assert torch.allclose(a, b, rtol=1e-5, atol=1e-5 * float(b.abs().max()))

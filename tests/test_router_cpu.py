@@ -54,6 +54,32 @@ def test_balance_arguments(lib):
         assert call() == 7
 
 
+def test_misaligned_and_too_many(lib):
+    a, b, c = P(256), P(258), P(260)
+
+    def route(bias=None, ids=a, w=a, n=a, k=4, g=1, kg=1, score=0):
+        return lib.qmoe_route(a, 0, 64, bias, 4, 64, k, g, kg, 0, score, 5.0, ids, w, n, None)
+
+    assert route(bias=b) == 2 and route(ids=c) == 2 and route(w=b) == 2 and route(n=b) == 2
+    assert route(k=17, g=8, kg=2, score=1) == 1            # a softmax leaves 16 experts in two of eight groups
+
+    def back(ids=a, dw=a, dl=a, dt=0):
+        return lib.qmoe_route_backward(a, dt, 64, 4, 64, 4, 0, 0, 5.0, ids, dw, dl, None)
+
+    assert back(ids=c) == 2 and back(dw=b) == 2 and back(dl=b) == 2 and back(dl=P(257), dt=1) == 2
+
+    def balance(T=100, k=22, loss=a, n=a, coef=a):
+        return lib.qmoe_balance(a, 0, 64, a, 1, None, T, 64, k, 0, 1.0, loss, n, coef, a, 1 << 30, None)
+
+    assert balance(loss=b) == 2 and balance(n=b) == 2 and balance(coef=b) == 2
+    assert balance(T=1 << 30, k=2) == 1                    # 2^31 ids: a count may pass 32 bits
+    assert lib.qmoe_balance_backward(a, 0, 64, None, 4, 64, 0, b, a, a, None) == 2
+    assert lib.qmoe_balance_backward(a, 0, 64, None, 4, 64, 0, a, b, a, None) == 2
+    assert lib.qmoe_balance_backward(a, 1, 64, None, 4, 64, 0, a, a, P(257), None) == 2
+    if not torch.cuda.is_available():
+        assert route() == 7 and route(k=16, g=8, kg=2, score=1) == 7 and back() == 7 and balance() == 7
+
+
 def test_python_refusals():
     import _qmoe_lib as C
     import router as R
