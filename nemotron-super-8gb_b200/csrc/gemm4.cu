@@ -359,8 +359,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 // more hand-offs per stage.) What bounds it is the tensor pipe at the clock the power limit leaves: 8192 x 12288 x
 // 4096 runs at 5.3 PFLOP/s, 0.78 of four times the bf16 rate of the library's product, and a version without any loads
 // took 0.96 of the time of the same version with them.
+// TN = 320 is for products of at most one tile per pair: one accumulator, two MMAs (192 and 128 columns) per k-step.
 template <int TN> struct PairPlan {
     static constexpr int NA = (TN + 127) / 128;
+    static constexpr int N0 = TN > 256 ? 192 : TN, N1 = TN - N0;   // columns of an MMA, of a second one
+    static constexpr int BOX = N1 ? 32 : TN / 2;                   // token or weight rows of a copy
     static constexpr int B_BYTES = TN / 2 * ROWB;
     static constexpr int OFF_B = A_BYTES, OFF_SFA = OFF_B + B_BYTES, OFF_SFB = OFF_SFA + SFA_BYTES;
     static constexpr int BYTES = OFF_SFB + NA * SFA_BYTES;
@@ -374,7 +377,7 @@ template <int TN> struct PairPlan {
     static_assert(SMEM <= 232448, "fits the 227 KB opt-in");
     // Tensor memory: two accumulators and two k-steps of scales. At TN = 256 the accumulators share 32 columns, which the
     // epilogue reads first, so that the next tile's MMAs wait for those alone; else for the tile before the last.
-    static constexpr int ACC1 = TN == 256 ? 224 : TN;
+    static constexpr int ACC1 = N1 ? 0 : TN == 256 ? 224 : TN;
     static constexpr int SF_COL = ACC1 + TN;
     static constexpr int SF_SLOT = 4 * (1 + NA);
     static constexpr int LAG = TN == 256 ? 1 : 2;
@@ -574,7 +577,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (elect_one()) {
                         if (rank == 0) mbar_expect_tx(&full[s], 2 * P::BYTES);
                         tma_load_2d_pair(st, &tm_a, kt * ROWB, a0, bar);
-                        tma_load_2d_pair(st + P::OFF_B, &tm_b, kt * ROWB, b0 + rank * (TN / 2), bar);
+#pragma unroll
+                        for (int r = 0; r < P::N0 / 2; r += P::BOX) tma_load_2d_pair(st + P::OFF_B + r * ROWB, &tm_b, kt * ROWB, b0 + rank * (P::N0 / 2) + r, bar);
+#pragma unroll
+                        for (int r = 0; r < P::N1 / 2; r += P::BOX)
+                            tma_load_2d_pair(st + P::OFF_B + (P::N0 / 2 + r) * ROWB, &tm_b, kt * ROWB, b0 + P::N0 + rank * (P::N1 / 2) + r, bar);
                         tma_load_2d_pair(st + P::OFF_SFA, &tm_sa, 0, fa + 4 * kt, bar);
 #pragma unroll
                         for (int a = 0; a < P::NA; a++)
@@ -588,7 +595,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     } else if (warp == 5) {
         // ------------------------------------------------------------ the first CTA's warp drives both tensor cores
         if (rank == 0) {
-            const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | (16u << 24);   // M = 256
+            constexpr uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(P::N0 >> 3) << 17) | (16u << 24);    // M = 256
+            constexpr uint32_t idesc1 = (1u << 7) | (1u << 10) | ((uint32_t)(P::N1 >> 3) << 17) | (16u << 24);
             const bool lead = elect_one();
             const int tail = p.nks - 4 * (p.nst - 1);   // k-steps of a tile's last stage
             uint32_t ph = 0;                            // parity of stage s's current use
@@ -596,7 +604,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             bool ok = true;
             for (int i = first; i < p.ntiles && ok; i += step, t++) {
                 const uint32_t d = (t & 1) * P::ACC1;
-                const uint32_t off = (uint32_t)(i / p.nba * TN & 127) >> 5;   // TN = 192: a tile may start at row 64 of an atom
+                const uint32_t off = (uint32_t)(i / p.nba * TN & 127) >> 5;   // TN = 192, 320: a tile may start at row 64 of an atom
                 for (int kt = 0; kt < p.nst; kt++) {
                     if (!all_wait(&full[s], ph, abort_flag, p.wait)) {
                         ok = false;
@@ -622,6 +630,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                     auto mma = [&](uint32_t at, int k, uint32_t acc) {
                         const uint32_t c = P::SF_COL + (k & 1) * P::SF_SLOT;
                         mma_pair(d, at + 2 * k, at + (P::OFF_B >> 4) + 2 * k, idesc, acc, c, c + 4 + off);
+                        if constexpr (P::N1 > 0)
+                            mma_pair(d + P::N0, at + 2 * k, at + ((P::OFF_B + P::N0 / 2 * ROWB) >> 4) + 2 * k, idesc1, acc, c, c + 4 + off + P::N0 / 32);
                     };
                     if (lead) {
                         copies(0);
@@ -811,7 +821,7 @@ static int launch_pair(const Params &g, const uint8_t *w, const uint8_t *x, int6
     p.y = g.y;
     p.wait = g.wait;
     CUtensorMap a, b, sa, sb;
-    if (!code_map(&a, t ? x : w, p.A, bytes, 128) || !code_map(&b, t ? w : x, p.B, bytes, TN / 2) ||
+    if (!code_map(&a, t ? x : w, p.A, bytes, 128) || !code_map(&b, t ? w : x, p.B, bytes, PairPlan<TN>::BOX) ||
         !atom_map(&sa, t ? g.sfb : g.sfa, p.A, p.nks) || !atom_map(&sb, t ? g.sfa : g.sfb, p.B, p.nks))
         return QMOE_ERR_LAUNCH;
     if (!(done.load(std::memory_order_acquire) >> (dev & 63) & 1) && !ensure_smem(kern, PairPlan<TN>::SMEM, dev, done)) return QMOE_ERR_LAUNCH;
@@ -845,8 +855,9 @@ static int launch_pair(const Params &p, const uint8_t *w, const uint8_t *x, int6
 
 // Up to 64 tokens: one tile of weight rows x all tokens per CTA, the stages split over a cluster where tiles are few. More:
 // pairs, with the columns that take the least time: waves of tiles times a tile's time, 1, 0.86 and 0.72 for 256, 192
-// and 128 columns (8192 x 12288 x 4096 in 155, 178 and 223 us). 2048 x 2688 x 4096: 19.6, 18.6, 23.0 us, 192 taken;
-// 128 x 4096 x 4096: 12.1, 11.5, 10.9, 128 taken (a cluster per tile of 128 x 128: 11.7).
+// and 128 columns (8192 x 12288 x 4096 in 155, 178 and 223 us); 128 x 4096 x 4096: 12.1, 11.5, 10.9, 128 taken (a cluster
+// per tile of 128 x 128: 11.7). 320 columns (1.25) where they make one wave and the others two: 2048 x 2688 x 4096 in
+// 12.7 us instead of 16.0 with 192, 512 x 10000 x 4096 in 12.0 instead of 15.3.
 template <typename T>
 static int pick(const Params &p, const CUtensorMap &a, const uint8_t *w, const uint8_t *x, int64_t bytes, cudaStream_t st, int dev, const DeviceInfo &di) {
     if (p.M <= 16) return launch<16, T>(p, a, x, bytes, st, dev, di);
@@ -854,7 +865,8 @@ static int pick(const Params &p, const CUtensorMap &a, const uint8_t *w, const u
     if (p.M <= 64) return launch<64, T>(p, a, x, bytes, st, dev, di);
     const int64_t A = tokens_on_lanes<T>(p) ? p.M : p.N, B = tokens_on_lanes<T>(p) ? p.N : p.M, pairs = di.sms / 2;
     auto cost = [&](int tn, int each) { return ((A + 255) / 256 * ((B + tn - 1) / tn) + pairs - 1) / pairs * each; };
-    const int64_t c128 = cost(128, 72), c192 = cost(192, 86), c256 = cost(256, 100);
+    const int64_t c128 = cost(128, 72), c192 = cost(192, 86), c256 = cost(256, 100), c320 = cost(320, 125);
+    if (c320 == 125 && c320 < c128 && c320 < c192 && c320 < c256) return launch_pair<320, T>(p, w, x, bytes, st, dev, di);
     if (c128 <= c192 && c128 <= c256) return launch_pair<128, T>(p, w, x, bytes, st, dev, di);
     if (c192 <= c256) return launch_pair<192, T>(p, w, x, bytes, st, dev, di);
     return launch_pair<256, T>(p, w, x, bytes, st, dev, di);

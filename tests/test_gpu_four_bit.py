@@ -366,3 +366,20 @@ def test_two_streams_at_once():
                 got += [(j, D.qlinear_a4(q, xs[j])) for j in (range(len(xs)) if i else reversed(range(len(xs))))]
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[j]) for j, y in got) and D.gemm_status() == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(2048, 2688, 512), (512, 10000, 96), (300, 11000, 288), (600, 9001, 320), (577, 9001, 32)])
+def test_gemm_in_one_wave_of_wide_tiles(M, N, K):
+    """Sizes whose tiles of 256 x 320 are one per pair of SMs: tiles that start inside an atom, end in their first part or
+    a few columns later, rows of y that are not aligned; the three types and epilogues, exact."""
+    import dense_q as D
+    g = seeded(M + N + K)
+    xq, q = D.prepare(small_integers(g, M, K)), D.prepare(small_integers(g, N, K))
+    ref = (values_of(xq) @ values_of(q).t()).float()
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        base = ref.to(dtype)
+        res = torch.randint(-8, 8, (M, N), generator=g, device=DEV).to(dtype)
+        assert torch.equal(D.gemm(q, xq, dtype), base)
+        assert torch.equal(D.gemm(q, xq, dtype, act="relu2"), (torch.relu(base.float()) ** 2).to(dtype))
+        assert torch.equal(D.gemm(q, xq, dtype, residual=res), (base.float() + res.float()).to(dtype))
+    assert D.gemm_status() == 0
