@@ -299,7 +299,8 @@ py::tuple route(const Tensor &logits, OptTensor bias, int64_t top_k, double scal
     return py::make_tuple(ids, w, n);
 }
 
-// Loss, counts, and coef * f / T' per expert for the backward pass.
+// Loss, counts, and a buffer that begins with coef * f / T' per expert, for the backward pass; the rest of it, 0.6 MB at
+// most, is the call's workspace (an allocation of its own costs more than a microsecond).
 std::tuple<Tensor, Tensor, Tensor> run_balance(const Tensor &x0, const Tensor &ids, const OptTensor &mask, int score, double coef) {
     int64_t ld;
     const Tensor x = rows_of(x0, ld);
@@ -309,11 +310,10 @@ std::tuple<Tensor, Tensor, Tensor> run_balance(const Tensor &x0, const Tensor &i
         const auto f = x.options().dtype(at::kFloat).requires_grad(false);
         return {at::zeros({}, f), at::zeros({E}, f.dtype(at::kInt)), at::zeros({E}, f)};
     }
-    const Tensor loss = empty({}, x, at::kFloat), n = empty({E}, x, at::kInt), c = empty({E}, x, at::kFloat);
-    const int64_t bytes = (int64_t)qmoe_balance_workspace_bytes(T, (int)E);
-    const Tensor ws = empty({bytes}, x, at::kByte);
+    const size_t bytes = qmoe_balance_workspace_bytes(T, (int)E);
+    const Tensor loss = empty({}, x, at::kFloat), n = empty({E}, x, at::kInt), c = empty({E + (int64_t)(bytes / 4)}, x, at::kFloat);
     status(qmoe_balance(data(x), dtype_code(x.scalar_type()), ld, data(ids), ids.scalar_type() == at::kLong, data<uint8_t>(mask), T, (int)E,
-                        (int)ids.size(1), score, (float)coef, data<float>(loss), data<int32_t>(n), data<float>(c), data(ws), (size_t)bytes, stream_of(x)), "qmoe_balance");
+                        (int)ids.size(1), score, (float)coef, data<float>(loss), data<int32_t>(n), data<float>(c), data<float>(c) + E, bytes, stream_of(x)), "qmoe_balance");
     return {loss, n, c};
 }
 

@@ -43,6 +43,40 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+// Clusters: a barrier of all threads that makes shared memory visible, and a word of CTA `rank`'s shared memory.
+constexpr int CLUSTER = 8;
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t word_of(const void *p, int rank) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.b32 %0, [r];\n\t}"
+                 : "=r"(v) : "r"(smem_u32(p)), "r"(rank) : "memory");
+    return v;
+}
+// A launch as clusters of n CTAs; pdl: it may begin before the kernel in front of it has ended (and waits in it).
+template <typename K, typename A>
+static int launch_cluster(K kern, unsigned grid, int threads, size_t smem, int n, bool pdl, cudaStream_t st, const A &a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)n;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, kern, a) != cudaSuccess) {
+        cudaGetLastError();
+        return QMOE_ERR_LAUNCH;
+    }
+    return launch_status();
+}
+
 // torch's fp32 sigmoid, bit for bit (expf, IEEE division).
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
 
@@ -128,6 +162,7 @@ struct Route {
     const float *bias;   // may be null
     int64_t T;
     int ne, k, n_group, topk_group, norm, softmax, vec;
+    int cluster;         // the CTAs are one cluster
     float scaling;
     int64_t *ids;        // [T, k]
     float *w;            // [T, k]
@@ -321,7 +356,9 @@ __device__ __forceinline__ void choose(const Route &a, int64_t t, int lane, cons
 
 // blockDim.x / 32 tokens at a time, up to ROUTE_WARPS. Every CTA adds its counts to the global ones at its end, so many
 // tokens take one large CTA per SM, up to 20 tokens per SM small CTAs of WARPS, up to four per SM (T x 512, small against
-// large: 1184 tokens 8.3 and 10.4 us, 2960 12.2 and 12.4, 4736 14.4 and 11.8, 37888 47 and 42).
+// large: 1184 tokens 8.3 and 10.4 us, 2960 12.2 and 12.4, 4736 14.4 and 11.8, 37888 47 and 42). What CLUSTER small
+// CTAs hold at a token per warp is one cluster, whose CTAs add up each other's counts: no clearing before the launch (64 x
+// 512: 6.3 and 4.7 us; with CLUSTER large CTAs 256 tokens took 7.5 instead of 6.3).
 template <int EPL> constexpr int ROUTE_WARPS = EPL > 16 ? 16 : 32;
 template <typename T, int EPL, bool FAST> __global__ void __launch_bounds__(ROUTE_WARPS<EPL> * 32) route_kernel(const Route a) {
     constexpr int SLOTS = EPL * 32;
@@ -365,6 +402,16 @@ template <typename T, int EPL, bool FAST> __global__ void __launch_bounds__(ROUT
             for (int i = 0; i < EPL; i++)
                 if (expert<EPL>(i, lane) >= a.ne) c[i] = -INFINITY;
         choose<EPL, FAST>(a, t, lane, c, v, bias, cand, hist);
+    }
+    if (a.cluster) {
+        cluster_sync();
+        for (int e = blockIdx.x * blockDim.x + threadIdx.x; e < a.ne; e += gridDim.x * blockDim.x) {
+            int n = 0;
+            for (int r = 0; r < (int)gridDim.x; r++) n += (int)word_of(&hist[e], r);
+            a.counts[e] = n;
+        }
+        cluster_sync();   // no CTA leaves while another reads its counts
+        return;
     }
     __syncthreads();
     const int turn = (int)(blockIdx.x * 96u % a.ne);   // CTAs that end together start at different experts
@@ -464,7 +511,31 @@ __device__ __forceinline__ void sigmoid_pair(float x, float &s, float &r) {
 // Its sigmoids may all underflow, their ratios need not.
 constexpr float LOW = 2e-9f;
 
-template <typename T, int EPL> __global__ void __launch_bounds__(BAL_WARPS<EPL> * 32) balance_kernel(const Balance a) {
+// Up to so many tokens per warp of CLUSTER CTAs are one kernel instead of two (256 x 512: 8.5 and 9.7 us, 512 x 512 10.0 and
+// 9.7, 1024 x 512 13.3 and 9.8; and a launch less for the host).
+constexpr int ONE_TOKENS = 2;
+
+// An expert's count and coefficient stored; its term of the loss.
+__device__ __forceinline__ float expert_term(const Balance &a, int e, float p, int n, int rows) {
+    const float f = rows ? (float)n * ((float)a.ne / ((float)a.k * (float)rows)) : 0.f;
+    a.counts[e] = n;
+    a.c[e] = rows ? a.coef * f / (float)rows : 0.f;
+    return rows ? f * (p / (float)rows) : 0.f;
+}
+
+// The sum of the CTAs' terms in their order, by the first one.
+__device__ __forceinline__ void store_loss(const Balance &a, const float *mine, int ctas) {
+    cluster_sync();
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        float sum = 0.f;
+        for (int i = 0; i < ctas; i++) sum += __uint_as_float(word_of(mine, i));
+        *a.loss = a.coef * sum;
+    }
+    cluster_sync();   // no CTA leaves before its term is read
+}
+
+// ONE: few tokens, all CTAs in one cluster, which adds their sums as well: no second kernel.
+template <typename T, int EPL, bool ONE> __global__ void __launch_bounds__(BAL_WARPS<EPL> * 32) balance_kernel(const Balance a) {
     constexpr int W = BAL_WARPS<EPL>;
     extern __shared__ float sm[];
     float *sums = sm;                                     // [W][ne]
@@ -522,15 +593,41 @@ template <typename T, int EPL> __global__ void __launch_bounds__(BAL_WARPS<EPL> 
         float p = 0.f;
 #pragma unroll
         for (int w = 0; w < W; w++) p += sums[w * a.ne + e];
-        a.part_p[(int64_t)blockIdx.x * a.ne + e] = p;
+        if (ONE) sums[e] = p;   // column e is this thread's alone
+        else a.part_p[(int64_t)blockIdx.x * a.ne + e] = p;
     }
-    for (int e = threadIdx.x; e <= a.ne; e += W * 32) a.part_n[(int64_t)blockIdx.x * (a.ne + 1) + e] = hist[e];
+    if constexpr (ONE) {
+        __shared__ float red[W], mine;
+        cluster_sync();
+        rows = 0;
+        for (int r = 0; r < a.parts; r++) rows += (int)word_of(&hist[a.ne], r);
+        float term = 0.f;
+        for (int e = blockIdx.x * W * 32 + threadIdx.x; e < a.ne; e += a.parts * W * 32) {
+            float p = 0.f;
+            int n = 0;
+            for (int r = 0; r < a.parts; r++) {
+                p += __uint_as_float(word_of(&sums[e], r));
+                n += (int)word_of(&hist[e], r);
+            }
+            term += expert_term(a, e, p, n, rows);
+        }
+        term = warp_sum(term);
+        if (lane == 0) red[warp] = term;
+        __syncthreads();
+        if (warp == 0) {
+            term = warp_sum(lane < W ? red[lane] : 0.f);
+            if (lane == 0) mine = term;
+        }
+        store_loss(a, &mine, a.parts);
+    } else {
+        for (int e = threadIdx.x; e <= a.ne; e += W * 32) a.part_n[(int64_t)blockIdx.x * (a.ne + 1) + e] = hist[e];
+    }
 }
 
 // The parts' sums: a cluster of FIN CTAs, each every FIN-th run of 32 experts, 32 rows of parts at a time (one CTA with a
 // thread per expert took 250 us for 592 parts). Every sum runs in a fixed order.
-constexpr int FIN = 8;
-__global__ void __launch_bounds__(1024) __cluster_dims__(FIN, 1, 1) balance_final_kernel(const Balance a) {
+constexpr int FIN = CLUSTER;
+__global__ void __launch_bounds__(1024) balance_final_kernel(const Balance a) {
     __shared__ float sp[32][33];
     __shared__ int sn[32][33];
     __shared__ int rows_of[32];
@@ -560,12 +657,7 @@ __global__ void __launch_bounds__(1024) __cluster_dims__(FIN, 1, 1) balance_fina
         // warp y sums expert e0 + y over the 32 rows
         p = warp_sum(sp[lane][y]);
         n = __reduce_add_sync(0xffffffffu, sn[lane][y]);
-        if (lane == 0 && e0 + y < a.ne) {
-            const float f = rows ? (float)n * ((float)a.ne / ((float)a.k * (float)rows)) : 0.f;
-            a.counts[e0 + y] = n;
-            a.c[e0 + y] = rows ? a.coef * f / (float)rows : 0.f;
-            term += rows ? f * (p / (float)rows) : 0.f;
-        }
+        if (lane == 0 && e0 + y < a.ne) term += expert_term(a, e0 + y, p, n, rows);
         __syncthreads();
     }
     if (lane == 0) sp[0][y] = term;
@@ -574,18 +666,7 @@ __global__ void __launch_bounds__(1024) __cluster_dims__(FIN, 1, 1) balance_fina
         term = warp_sum(sp[0][lane]);
         if (lane == 0) mine = term;
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank == 0 && threadIdx.x == 0) {
-        float sum = 0.f;
-        for (int i = 0; i < FIN; i++) {
-            float v;
-            asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}"
-                         : "=f"(v) : "r"(smem_u32(&mine)), "r"(i) : "memory");
-            sum += v;
-        }
-        *a.loss = a.coef * sum;
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    store_loss(a, &mine, FIN);
 }
 
 template <typename T, int EPL> __global__ void __launch_bounds__(THREADS, EPL > 16 ? 2 : 4) balance_backward_kernel(const Balance a) {
@@ -717,10 +798,12 @@ int qmoe_route(const void *logits, int x_dtype, int64_t ld, const float *bias, i
         using X = decltype(t);
         const int warps = T <= (int64_t)di->sms * 20 ? rt::WARPS : rt::ROUTE_WARPS<EPL>;
         const int64_t ctas = (T + warps - 1) / warps;
+        a.cluster = ctas > 1 && ctas <= rt::CLUSTER;
         const unsigned grid = (unsigned)(ctas < di->sms * (warps == rt::WARPS ? 4 : 1) ? ctas : di->sms * (warps == rt::WARPS ? 4 : 1));
         const size_t smem = warps * sizeof(rt::Candidates) + sizeof(float) * (EPL * 32 + n_experts * (n_group > 1 ? 1 + warps : 1));
         auto launch = [&](auto kern, std::atomic<uint64_t> &done) -> int {
             if (!(done.load(std::memory_order_acquire) >> (dev & 63) & 1) && !ensure_smem(kern, smem, dev, done)) return QMOE_ERR_LAUNCH;
+            if (a.cluster) return rt::launch_cluster(kern, grid, warps * 32, smem, (int)grid, false, st, a);
             if (grid > 1 && cudaMemsetAsync(counts, 0, sizeof(int) * n_experts, st) != cudaSuccess) return QMOE_ERR_LAUNCH;
             kern<<<grid, warps * 32, smem, st>>>(a);
             return launch_status();
@@ -798,30 +881,21 @@ int qmoe_balance(const void *logits, int x_dtype, int64_t ld, const void *ids, i
     a.part_p = static_cast<float *>(workspace);
     a.part_n = static_cast<int *>(workspace) + (int64_t)a.parts * n_experts;
     cudaStream_t st = as_stream(stream);
-    const int rc = rt::by_type(x_dtype, n_experts, [&](auto t, auto w) {
-        static std::atomic<uint64_t> done{0};
-        constexpr int W = rt::BAL_WARPS<decltype(w)::value>;
-        auto kern = rt::balance_kernel<decltype(t), decltype(w)::value>;
+    const bool one = T <= rt::ONE_TOKENS * rt::CLUSTER * warps;
+    if (one && a.parts > rt::CLUSTER) a.parts = rt::CLUSTER;
+    const int rc = rt::by_type(x_dtype, n_experts, [&](auto t, auto w) -> int {
+        static std::atomic<uint64_t> done_one{0}, done_parts{0};
+        using X = decltype(t);
+        constexpr int EPL = decltype(w)::value, W = rt::BAL_WARPS<EPL>;
         const size_t smem = sizeof(float) * ((W + 1) * n_experts + 1);   // at most 68 KB
-        if (!(done.load(std::memory_order_acquire) >> (dev & 63) & 1) && !ensure_smem(kern, smem, dev, done)) return QMOE_ERR_LAUNCH;
-        kern<<<a.parts, W * 32, smem, st>>>(a);
-        return launch_status();
+        auto launch = [&](auto kern, std::atomic<uint64_t> &done) -> int {
+            if (!(done.load(std::memory_order_acquire) >> (dev & 63) & 1) && !ensure_smem(kern, smem, dev, done)) return QMOE_ERR_LAUNCH;
+            return rt::launch_cluster(kern, (unsigned)a.parts, W * 32, smem, one ? a.parts : 1, false, st, a);
+        };
+        return one ? launch(rt::balance_kernel<X, EPL, true>, done_one) : launch(rt::balance_kernel<X, EPL, false>, done_parts);
     });
-    if (rc) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(rt::FIN);
-    cfg.blockDim = dim3(1024);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, rt::balance_final_kernel, a) != cudaSuccess) {
-        cudaGetLastError();
-        return QMOE_ERR_LAUNCH;
-    }
-    return launch_status();
+    if (rc || one) return rc;
+    return rt::launch_cluster(rt::balance_final_kernel, rt::FIN, 1024, 0, rt::FIN, true, st, a);
 }
 
 int qmoe_balance_backward(const void *logits, int x_dtype, int64_t ld, const uint8_t *mask, int64_t T, int n_experts,

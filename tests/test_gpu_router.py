@@ -420,7 +420,7 @@ def test_route_refusals():
             bad()
 
 
-@pytest.mark.parametrize("T", [1, 7, 8, 9, 2959, 2960, 2961, 3500, 4737])
+@pytest.mark.parametrize("T", [1, 7, 8, 9, 63, 64, 65, 2959, 2960, 2961, 3500, 4737])
 def test_route_counts_at_the_launch_borders(T):
     check_route(torch.randn(T, 96, generator=seeded(T), device=DEV), None, 6, grad=False)
 
@@ -454,3 +454,15 @@ def test_backward_into_a_graph():
         step()
         for a, b in zip(got, (x.grad, gate.grad)):
             assert torch.allclose(a, b, rtol=1e-5, atol=1e-5 * float(b.abs().max()))
+
+
+@pytest.mark.parametrize("E", [96, 512, 1000])
+@pytest.mark.parametrize("T", [1, 16, 17, 31, 33, 255, 256, 257, 511, 512, 513])
+def test_balance_at_the_launch_borders(T, E):
+    """One CTA, a cluster with ragged parts, and the two kernels: loss, counts and gradient, masked and not."""
+    g = seeded(T + E)
+    x = torch.randn(T, E, generator=g, device=DEV)
+    ids = torch.randint(0, E, (T, 5), generator=g, device=DEV)
+    for mask in (None, torch.rand(T, generator=g, device=DEV) < 0.6):
+        for score in ("sigmoid", "softmax"):
+            check_balance(x, ids, mask, score, 0.5)
