@@ -68,6 +68,13 @@ template <typename T> __device__ __forceinline__ void widen(const Raw<T> &v, flo
 
 // fp32 bits of the largest finite magnitude of a block; with NONFINITE set where the block holds anything else.
 constexpr uint32_t NONFINITE = 0x80000000u;
+// The larger magnitudes of two pairs, NaN where either is; the signs are of no use.
+template <typename T> __device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 template <typename T> __device__ __forceinline__ uint32_t block_max(const Raw<T> &v) {
     uint32_t m = 0;
     if constexpr (sizeof(T) == 4) {
@@ -76,7 +83,8 @@ template <typename T> __device__ __forceinline__ uint32_t block_max(const Raw<T>
         if (m < 0x7F800000u) return m;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = __vmaxu2(m, v.r[i] & 0x7FFF7FFFu);
+        for (int i = 0; i < 8; i++) m = larger2<T>(m, v.r[i]);
+        m &= 0x7FFF7FFFu;
         m = max(m & 0xFFFFu, m >> 16);
         if (std::is_same<T, __half>::value && m < 0x7C00u) return __float_as_uint(__half2float(__ushort_as_half((uint16_t)m)));
         if (!std::is_same<T, __half>::value && m < 0x7F80u) return m << 16;
@@ -100,6 +108,14 @@ __device__ __forceinline__ int scale_exp(uint32_t bits) {
 // Round to odd at 13 significant bits (of a normal number's bits).
 __device__ __forceinline__ uint32_t odd13(uint32_t b) { return (b | ((b & 0x7FFu) + 0x7FFu)) & ~0x7FFu; }
 
+// a = a f + 192 - 192, each step rounded once, and b likewise: two elements per instruction.
+__device__ __forceinline__ void snap2(float &a, float &b, float f) {
+    asm("{\n\t.reg .b64 v, g, c, d;\n\t"
+        "mov.b64 v, {%0, %1};\n\tmov.b64 g, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\tmov.b64 d, {%4, %4};\n\t"
+        "fma.rn.f32x2 v, v, g, c;\n\tadd.rn.f32x2 v, v, d;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(f), "f"(192.f), "f"(-192.f));
+}
+
 // One block whose block_max is `top`: codes (element 2i in the low nibble of byte i) and scale byte, s = 2^e.
 template <typename T> __device__ __forceinline__ uint32_t block16(const Raw<T> &v, uint32_t top, int e, uint2 &codes) {
     codes = make_uint2(0u, 0u);
@@ -122,11 +138,12 @@ template <typename T> __device__ __forceinline__ uint32_t block16(const Raw<T> &
 #pragma unroll
         for (int i = 0; i < 16; i++) q[i] *= inv_s;
     }
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        if constexpr (sizeof(T) == 4) q[i] = __uint_as_float(odd13(__float_as_uint(q[i])));
-        q[i] = fmaf(q[i], f, 192.f) - 192.f;
+        for (int i = 0; i < 16; i++) q[i] = __uint_as_float(odd13(__float_as_uint(q[i])));
     }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) snap2(q[i], q[i + 1], f);
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         uint32_t &c = k ? codes.y : codes.x;
