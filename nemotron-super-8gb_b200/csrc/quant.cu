@@ -1,9 +1,9 @@
 // NVFP4 quantisation (dq_quantize_nvfp4), its inverse, and the tensor-core layout of block scales; the definition, and
 // how its decisions are exact, in quant.cuh.
 //
-// Bounds: bytes, 2.56 an element for bf16 (131072 x 4096: 231 us, 5.9 TB/s), and next to them issue, 13 to 14 instructions an
-// element. With IEEE divisions and a comparison per midpoint 16384 x 4096 bf16 took 61 us, now 36 (26 at the
-// copy rate); the inverse takes 27 to 31 us for the same elements.
+// Bounds: bytes, 2.56 an element for bf16 (131072 x 4096: 220 us, 6.25 TB/s), and next to them issue, 12 instructions an
+// element (ncu). With IEEE divisions and a comparison per midpoint 16384 x 4096 bf16 took 61 us, now 33 (26 at the copy
+// rate); the inverse takes 26 to 31 us for the same elements.
 #include "common.cuh"
 #include "host.h"
 #include "quant.cuh"
