@@ -120,6 +120,8 @@ def call(name, *args):
 
 def stream_of(t=None):
     """cudaStream_t of torch's current stream on the tensor's device."""
+    if t is not None and not t.is_cuda:
+        raise QmoeError("libqmoe_b200 works on CUDA tensors only (got a CPU tensor)")
     return torch._C._cuda_getCurrentRawStream(t.get_device() if t is not None else torch.cuda.current_device())
 
 

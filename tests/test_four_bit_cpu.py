@@ -139,3 +139,11 @@ def test_prepare_looks_at_the_weight():
                 {"sc": torch.zeros(4, 4)}, {"s": torch.ones(4)}, {"s": torch.ones(1, dtype=torch.float64)}, {"fmt": "nvfp4_rows"}, {}):
         with pytest.raises(C.QmoeError):
             D.prepare({**q, **bad})
+
+
+def test_a_cpu_tensor_has_no_stream():
+    import _qmoe_lib as C
+    import dense_q as D
+    q = {"fmt": "nvfp4", "w": torch.zeros(4, 32, dtype=torch.uint8), "sc": torch.zeros(4, 4, dtype=torch.uint8), "s": torch.ones(1), "N": 4, "K": 64}
+    with pytest.raises(C.QmoeError, match="CUDA tensors"):
+        D.gemv(q, torch.zeros(64))
