@@ -9,8 +9,12 @@
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/FunctionsManual.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/qmoe_b200.h"
@@ -235,6 +239,7 @@ Tensor once(const Tensor &g) {
 struct RouteArgs { int64_t k, n_group, topk_group; bool norm; int score; double scaling; };
 
 std::tuple<Tensor, Tensor, Tensor> run_route(const Tensor &x0, const OptTensor &bias, const RouteArgs &a) {
+    const at::AutoGradMode off(false);
     int64_t ld;
     const Tensor x = rows_of(x0, ld);
     const int64_t T = x.size(0), E = x.size(1);
@@ -247,34 +252,60 @@ std::tuple<Tensor, Tensor, Tensor> run_route(const Tensor &x0, const OptTensor &
     return {ids, w, n};
 }
 
-struct Route : torch::autograd::Function<Route> {
-    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &logits, const OptTensor &bias, int64_t k,
-                                                  int64_t n_group, int64_t topk_group, bool norm, int64_t score, double scaling) {
-        auto [ids, w, n] = run_route(logits, bias, {k, n_group, topk_group, norm, (int)score, scaling});
-        ctx->save_for_backward({logits, ids});
-        ctx->saved_data["norm"] = norm;
-        ctx->saved_data["score"] = score;
-        ctx->saved_data["scaling"] = scaling;
-        ctx->mark_non_differentiable({ids, n});
-        ctx->set_materialize_grads(false);
-        return {ids, w, n};
+// The operators' gradients as nodes of torch's graph. (torch::autograd::Function, which converts every argument, took 62 us
+// for the loss of 200 tokens and its gradient; this 58, of which torch's engine is about 40.)
+struct Gradient : torch::autograd::Node {
+    torch::autograd::SavedVariable logits;
+    int score;
+    Gradient(const Tensor &x, int score) : Node(torch::autograd::collect_next_edges(x)), logits(x, false), score(score) {}
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        logits.reset_data();
     }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-        torch::autograd::variable_list out(8);
-        if (!grads[1].defined()) return out;
-        const auto saved = ctx->get_saved_variables();
-        int64_t ld;
-        const Tensor x = rows_of(saved[0], ld), &ids = saved[1];
-        const c10::cuda::CUDAGuard guard(x.device());
-        const Tensor dl = empty(x.sizes(), x, x.scalar_type());
-        if (x.size(0)) {
-            const Tensor dw = grads[1].to(at::kFloat).contiguous();
-            status(qmoe_route_backward(data(x), dtype_code(x.scalar_type()), ld, x.size(0), (int)x.size(1), (int)ids.size(1), ctx->saved_data["norm"].toBool(),
-                                       (int)ctx->saved_data["score"].toInt(), (float)ctx->saved_data["scaling"].toDouble(), data<int64_t>(ids),
-                                       data<float>(dw), data(dl), stream_of(x)), "qmoe_route_backward");
+    // d logits of the output's gradient g
+    virtual Tensor gradient(const Tensor &x, int64_t ld, const Tensor &g) = 0;
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) return {Tensor()};
+        Tensor dl;
+        {
+            const at::AutoGradMode off(false);
+            const Tensor saved = logits.unpack();
+            int64_t ld;
+            const Tensor x = rows_of(saved, ld);
+            const c10::cuda::CUDAGuard guard(x.device());
+            dl = gradient(x, ld, grads[0].to(at::kFloat));
         }
-        out[0] = once(dl);
-        return out;
+        return {once(dl)};
+    }
+};
+
+// `out` becomes the output whose gradient the node takes.
+void attach(const Tensor &out, std::shared_ptr<torch::autograd::Node> node) { torch::autograd::set_history(out, node); }
+
+bool differentiated(const Tensor &x) {
+    if (!at::GradMode::is_enabled()) return false;
+    REQUIRE(!torch::autograd::isFwGradDefined(x), "the router's operators have no forward-mode derivative");
+    return x.requires_grad();
+}
+
+struct RouteBackward : Gradient {
+    torch::autograd::SavedVariable ids;
+    bool norm;
+    double scaling;
+    RouteBackward(const Tensor &x, const Tensor &ids, const RouteArgs &a) : Gradient(x, a.score), ids(ids, false), norm(a.norm), scaling(a.scaling) {}
+    std::string name() const override { return "RouteBackward"; }
+    void release_variables() override {
+        Gradient::release_variables();
+        std::lock_guard<std::mutex> lock(mutex_);
+        ids.reset_data();
+    }
+    Tensor gradient(const Tensor &x, int64_t ld, const Tensor &g) override {
+        const Tensor dl = empty(x.sizes(), x, x.scalar_type()), i = ids.unpack(), dw = g.contiguous();
+        if (x.size(0))
+            status(qmoe_route_backward(data(x), dtype_code(x.scalar_type()), ld, x.size(0), (int)x.size(1), (int)i.size(1), norm, score, (float)scaling,
+                                       data<int64_t>(i), data<float>(dw), data(dl), stream_of(x)), "qmoe_route_backward");
+        return dl;
     }
 };
 
@@ -291,17 +322,16 @@ py::tuple route(const Tensor &logits, OptTensor bias, int64_t top_k, double scal
         REQUIRE(bias->dim() == 1 && bias->size(0) == E && bias->device() == logits.device(), "bias must be [E], on the logits' device");
         bias = bias->detach().to(at::kFloat).contiguous();
     }
-    if (logits.requires_grad() && at::GradMode::is_enabled()) {
-        const auto r = Route::apply(logits, bias, top_k, n_group, topk_group, norm, (int64_t)sc, scaling);
-        return py::make_tuple(r[0], r[1], r[2]);
-    }
-    auto [ids, w, n] = run_route(logits, bias, {top_k, n_group, topk_group, norm, sc, scaling});
+    const RouteArgs args{top_k, n_group, topk_group, norm, sc, scaling};
+    auto [ids, w, n] = run_route(logits, bias, args);
+    if (differentiated(logits)) attach(w, std::shared_ptr<RouteBackward>(new RouteBackward(logits, ids, args), torch::autograd::deleteNode));
     return py::make_tuple(ids, w, n);
 }
 
 // Loss, counts, and a buffer that begins with coef * f / T' per expert, for the backward pass; the rest of it, 0.6 MB at
 // most, is the call's workspace (an allocation of its own costs more than a microsecond).
 std::tuple<Tensor, Tensor, Tensor> run_balance(const Tensor &x0, const Tensor &ids, const OptTensor &mask, int score, double coef) {
+    const at::AutoGradMode off(false);
     int64_t ld;
     const Tensor x = rows_of(x0, ld);
     const int64_t T = x.size(0), E = x.size(1);
@@ -317,32 +347,22 @@ std::tuple<Tensor, Tensor, Tensor> run_balance(const Tensor &x0, const Tensor &i
     return {loss, n, c};
 }
 
-struct Balance : torch::autograd::Function<Balance> {
-    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &logits, const Tensor &ids, const OptTensor &mask,
-                                                  int64_t score, double coef) {
-        auto [loss, n, c] = run_balance(logits, ids, mask, (int)score, coef);
-        ctx->save_for_backward({logits, c, mask ? *mask : Tensor()});
-        ctx->saved_data["score"] = score;
-        ctx->mark_non_differentiable({n});
-        ctx->set_materialize_grads(false);
-        return {loss, n};
+struct BalanceBackward : Gradient {
+    torch::autograd::SavedVariable c, mask;
+    BalanceBackward(const Tensor &x, const Tensor &c, const OptTensor &mask, int score) : Gradient(x, score), c(c, false), mask(mask ? *mask : Tensor(), false) {}
+    std::string name() const override { return "BalanceBackward"; }
+    void release_variables() override {
+        Gradient::release_variables();
+        std::lock_guard<std::mutex> lock(mutex_);
+        c.reset_data();
+        mask.reset_data();
     }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-        torch::autograd::variable_list out(5);
-        if (!grads[0].defined()) return out;
-        const auto saved = ctx->get_saved_variables();
-        int64_t ld;
-        const Tensor x = rows_of(saved[0], ld);
-        const c10::cuda::CUDAGuard guard(x.device());
-        const Tensor dl = empty(x.sizes(), x, x.scalar_type());
-        if (x.size(0)) {
-            const Tensor g = grads[0].to(at::kFloat);
-            const OptTensor mask = saved[2].defined() ? OptTensor(saved[2]) : OptTensor();
-            status(qmoe_balance_backward(data(x), dtype_code(x.scalar_type()), ld, data<uint8_t>(mask), x.size(0), (int)x.size(1),
-                                         (int)ctx->saved_data["score"].toInt(), data<float>(saved[1]), data<float>(g), data(dl), stream_of(x)), "qmoe_balance_backward");
-        }
-        out[0] = once(dl);
-        return out;
+    Tensor gradient(const Tensor &x, int64_t ld, const Tensor &g) override {
+        const Tensor dl = empty(x.sizes(), x, x.scalar_type()), m = mask.unpack();
+        if (x.size(0))
+            status(qmoe_balance_backward(data(x), dtype_code(x.scalar_type()), ld, m.defined() ? data<uint8_t>(m) : nullptr, x.size(0), (int)x.size(1), score,
+                                         data<float>(c.unpack()), data<float>(g), data(dl), stream_of(x)), "qmoe_balance_backward");
+        return dl;
     }
 };
 
@@ -360,11 +380,8 @@ py::tuple balance_loss(const Tensor &logits, const Tensor &ids0, OptTensor mask,
                 "mask must be bool [T], on the logits' device");
         mask = mask->contiguous();
     }
-    if (logits.requires_grad() && at::GradMode::is_enabled()) {
-        const auto r = Balance::apply(logits, ids, mask, (int64_t)sc, coef);
-        return py::make_tuple(r[0], r[1]);
-    }
     auto [loss, n, c] = run_balance(logits, ids, mask, sc, coef);
+    if (differentiated(logits)) attach(loss, std::shared_ptr<BalanceBackward>(new BalanceBackward(logits, c, mask, sc), torch::autograd::deleteNode));
     return py::make_tuple(loss, n);
 }
 

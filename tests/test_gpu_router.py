@@ -466,3 +466,52 @@ def test_balance_at_the_launch_borders(T, E):
     for mask in (None, torch.rand(T, generator=g, device=DEV) < 0.6):
         for score in ("sigmoid", "softmax"):
             check_balance(x, ids, mask, score, 0.5)
+
+
+def test_graphs_that_are_used_twice_or_changed():
+    import _qmoe_lib as C
+    import router as R
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(20, 32, generator=seeded(61), device=DEV, requires_grad=True)
+    for f in (lambda v: R.route(v, None, top_k=3)[1].square().sum(),
+              lambda v: R.balance_loss(v, torch.topk(v.detach(), 3)[1], torch.ones(20, dtype=torch.bool, device=DEV))[0]):
+        out = f(x)
+        a, = torch.autograd.grad(out, x, retain_graph=True)
+        b, = torch.autograd.grad(out, x)
+        assert torch.equal(a, b)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(out, x)
+        y = x * 1.0
+        out = f(y)
+        y.mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad(out, x)
+        with fwd.dual_level(), pytest.raises(C.QmoeError, match="forward-mode"):
+            f(fwd.make_dual(x.detach(), torch.ones_like(x)))
+    ids, w, _ = R.route(x, None, top_k=3)
+    ids.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(w.sum(), x)
+
+
+def test_gradients_of_views_and_copies():
+    """Logits that are views, broadcast over tokens or strided: the gradient has their shape, and sums where they share."""
+    import router as R
+    g = seeded(62)
+    row = torch.randn(1, 48, generator=g, device=DEV, requires_grad=True)
+    wide = torch.randn(30, 96, generator=g, device=DEV, requires_grad=True)
+    ids = torch.randint(0, 48, (30, 4), generator=g, device=DEV)
+    for leaf, view in ((row, lambda v: v.expand(30, 48)), (wide, lambda v: v[:, 3:51]), (wide, lambda v: v[:, ::2]), (wide, lambda v: v.t()[:30, :30])):
+        def both(z, make):
+            n = z.shape[1]
+            i = ids % n
+            return make(z, i)
+        got, = torch.autograd.grad(both(view(leaf), lambda z, i: R.balance_loss(z, i)[0]), leaf)
+        y = leaf.detach().double().requires_grad_()
+        want, = torch.autograd.grad(both(view(y), lambda z, i: loss64(z, i, None, "sigmoid", 1.0)[0]), y)
+        assert got.shape == leaf.shape and bool(((got.double() - want).abs() <= 4 * TOL * want.abs().max()).all())
+        dw = torch.randn(view(leaf).shape[0], 4, generator=seeded(5), device=DEV)
+        chosen_ids, w, _ = R.route(view(leaf), None, top_k=4)
+        got, = torch.autograd.grad(w, leaf, dw)
+        want, = torch.autograd.grad(weights64(view(y), chosen_ids, 5.0, False, "sigmoid"), y, dw.double())
+        assert bool(((got.double() - want).abs() <= TOL * 5 * dw.abs().double().sum()).all())
