@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(THREADS) tensor_kernel(const Args a) {
 template <typename T>
 static int launch(const Args &a, bool per_row, cudaStream_t st, const DeviceInfo &di) {
     if (per_row) {
-        // the fewest threads whose registers hold a row, or more while the rows leave room on the SMs
+        // the fewest threads whose registers hold a row, or more while the rows leave room on the SMs (bf16 x 4096, caches
+        // cold, 32, 64, 128 and 256 threads: 8192 rows 26.0, 20.3, 22.5, 28.8 us; 512 rows 8.5, 4.3, 3.8, 3.6)
         int g = 32;
         while (g < THREADS && (a.nb > g * KEEP || (a.nb > g && a.M * g * 2 <= (int64_t)di.sms * 1024))) g *= 2;
         const unsigned grid = (unsigned)((a.M + THREADS / g - 1) / (THREADS / g));
