@@ -548,14 +548,14 @@ template <typename T, int EPL, bool ONE> __global__ void __launch_bounds__(BAL_W
     for (int i = 0; i < EPL; i++) acc[i] = 0.f;
     int rows = 0;
     const int64_t step = (int64_t)gridDim.x * W;
-    uint32_t live = ~0u;   // masks of the warp's next 32 tokens, fetched together
+    uint32_t live = 0;   // masks of the warp's next 32 tokens, fetched together
     int left = 0;
     for (int64_t t = blockIdx.x * (int64_t)W + warp; t < a.T; t += step, live >>= 1, left--) {
         if (a.mask && left == 0) {
             live = __ballot_sync(0xffffffffu, t + lane * step < a.T && a.mask[t + lane * step]);
             left = 32;
         }
-        if (!(live & 1u)) continue;
+        if (a.mask && !(live & 1u)) continue;
         rows++;
         const T *row = static_cast<const T *>(a.logits) + t * a.ld;
         float s[EPL];
@@ -676,7 +676,7 @@ template <typename T, int EPL> __global__ void __launch_bounds__(THREADS, EPL > 
 #pragma unroll
     for (int i = 0; i < EPL; i++) c[i] = expert<EPL>(i, lane) < a.ne ? a.c[expert<EPL>(i, lane)] : 0.f;
     const int64_t step = (int64_t)gridDim.x * WARPS;
-    uint32_t live = ~0u;   // as in balance_kernel
+    uint32_t live = 0;   // as in balance_kernel
     int left = 0;
     for (int64_t t = blockIdx.x * (int64_t)WARPS + (threadIdx.x >> 5); t < a.T; t += step, live >>= 1, left--) {
         if (a.mask && left == 0) {
@@ -686,7 +686,7 @@ template <typename T, int EPL> __global__ void __launch_bounds__(THREADS, EPL > 
         T *out = static_cast<T *>(a.dl) + t * a.ne;
         const T *row = static_cast<const T *>(a.logits) + t * a.ld;
         float u[EPL];   // p before its division, times 1 - s
-        if (!(live & 1u)) {
+        if (a.mask && !(live & 1u)) {
 #pragma unroll
             for (int i = 0; i < EPL; i++) u[i] = 0.f;
             store_row<T, EPL>(out, a.ne, lane, a.vec, u);

@@ -515,3 +515,32 @@ def test_gradients_of_views_and_copies():
         got, = torch.autograd.grad(w, leaf, dw)
         want, = torch.autograd.grad(weights64(view(y), chosen_ids, 5.0, False, "sigmoid"), y, dw.double())
         assert bool(((got.double() - want).abs() <= TOL * 5 * dw.abs().double().sum()).all())
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("T,E", [(160001, 8), (320003, 16), (80001, 520), (155000, 1000)])
+def test_balance_of_batches_beyond_32_tokens_per_warp(T, E, masked):
+    """A warp fetches its masks for 32 tokens at a time: batches in which it has more of them, masked and not. An expert's sum
+    of p (positive terms) goes through at most T / 2368 additions of a warp (148 CTAs of 16 warps or more), 32 over the
+    warps, 5 over the parts of a thread and 5 of a tree, each off by 2^-24 of the sum at most: added to TOL. The
+    gradient has no sum over tokens."""
+    import router as R
+    g = seeded(T + E)
+    x = torch.randn(T, E, generator=g, device=DEV, requires_grad=True)
+    ids = torch.randint(0, E, (T, 2), generator=g, device=DEV)
+    mask = torch.rand(T, generator=g, device=DEV) < 0.7 if masked else None
+    keep = mask if masked else torch.ones(T, dtype=torch.bool, device=DEV)
+    for score in ("sigmoid", "softmax"):
+        loss, n = R.balance_loss(x, ids, mask, score, 0.5)
+        got, = torch.autograd.grad(loss, x)
+        y = x.detach().double()
+        want, n64, c = loss64(y, ids, mask, score, 0.5)
+        assert torch.equal(n, n64.to(torch.int32))
+        assert abs(float(loss.detach()) - float(want)) <= (TOL + (T / 2368 + 42) * 2.0 ** -24) * float(want)
+        s = torch.sigmoid(y) if score == "sigmoid" else torch.softmax(y, -1)
+        p = s / s.sum(-1, keepdim=True)
+        dot = (c * p).sum(-1, keepdim=True)
+        ref = p * (c - dot) * (1 - s if score == "sigmoid" else 1.0)
+        error = (got.double() - ref).abs() - TOL * p * (c + dot)
+        assert float(error[keep].max()) <= 0 and not got[~keep].any()
+        assert bool(got[keep][-1].any())
