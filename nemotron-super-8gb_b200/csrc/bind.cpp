@@ -97,6 +97,16 @@ void check_device(const Tensor &w, const Tensor &sc, const Tensor &s) {
     REQUIRE(w.is_cuda() && sc.device() == w.device() && s.device() == w.device(), "libqmoe_b200 works on CUDA tensors only, all of a weight on one device");
 }
 
+// The same for the inverse, which takes the bytes in any one-byte type and shape.
+void check_stored(const Tensor &w, const Tensor &sc, const Tensor &s, bool per_row, int64_t N, int64_t K) {
+    REQUIRE(N >= 0 && K >= 16 && K % 16 == 0, "a quantised matrix has rows of a positive multiple of 16 elements (got ", N, " x ", K, ")");
+    for (auto [name, t, bytes] : {std::make_tuple("w", &w, N * (K / 2)), std::make_tuple("sc", &sc, N * (K / 16))})
+        REQUIRE(t->element_size() == 1 && t->numel() == bytes && t->is_contiguous(), name, " must be ", bytes, " contiguous bytes for ", N, " rows of ", K, " elements");
+    REQUIRE(s.scalar_type() == at::kFloat && s.numel() == (per_row ? N : 1) && s.is_contiguous(),
+            "s must be float32, one value (nvfp4) or one per row (nvfp4_rows)");
+    check_device(w, sc, s);
+}
+
 int64_t atoms_bytes(int64_t rows, int64_t K) { return (rows + 127) / 128 * ((K + 63) / 64) * 512; }
 
 // A quantised matrix as a product's operand: its tensors, and its scale atoms where it has them.
@@ -135,7 +145,7 @@ py::tuple quantize(const Tensor &x0, bool per_row, bool for_gemm) {
 }
 
 Tensor dequant(const Tensor &w, const Tensor &sc, const Tensor &s, bool per_row, int64_t N, int64_t K) {
-    REQUIRE(w.is_cuda(), "libqmoe_b200 works on CUDA tensors only (got a CPU tensor)");
+    check_stored(w, sc, s, per_row, N, K);
     const c10::cuda::CUDAGuard guard(w.device());
     const Tensor out = empty({N, K}, w, at::kBFloat16);
     if (N && per_row) status(dq_dequant_nvfp4(data<uint8_t>(w), data<uint8_t>(sc), data<float>(s), 1, N, K, 0, N, data(out), QMOE_DT_BF16, stream_of(w)), "dq_dequant_nvfp4");
@@ -402,6 +412,7 @@ PYBIND11_MODULE(qmoe_torch, m) {
     });
     m.def("quantize", &quantize);
     m.def("scale_atoms", &scale_atoms);
+    m.def("check_stored", &check_stored);
     m.def("dequant", &dequant);
     m.def("gemm", &gemm);
     m.def("linear_a4", &linear_a4);

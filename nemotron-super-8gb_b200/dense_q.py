@@ -73,7 +73,10 @@ def dequant_rows(q, r0, r1, out):
         raise C.QmoeError("out must be contiguous")
     sc = q.get("sc")
     if q["fmt"] == "nvfp4_rows":
-        if r1 > r0:
+        C.bind().check_stored(q["w"], sc, q["s"], True, q["N"], q["K"])
+        if out.device != q["w"].device or out.numel() != (r1 - r0) * q["K"]:
+            raise C.QmoeError(f"out must be [{r1 - r0}, {q['K']}], on the matrix's device")
+        if r1 != r0:
             with torch.cuda.device(out.device):
                 C.call("dq_dequant_nvfp4", C.ptr(q["w"]), C.ptr(sc), C.ptr(q["s"]), 1, q["N"], q["K"], r0, r1, C.ptr(out),
                        C.dtype_code(out), C.stream_of(out))

@@ -147,3 +147,21 @@ def test_a_cpu_tensor_has_no_stream():
     q = {"fmt": "nvfp4", "w": torch.zeros(4, 32, dtype=torch.uint8), "sc": torch.zeros(4, 4, dtype=torch.uint8), "s": torch.ones(1), "N": 4, "K": 64}
     with pytest.raises(C.QmoeError, match="CUDA tensors"):
         D.gemv(q, torch.zeros(64))
+
+
+def test_the_inverse_looks_at_its_tensors():
+    """What is read has to be there: sizes, types and layout of every tensor, before any launch."""
+    import _qmoe_lib as C
+    import dense_q as D
+    one = {"fmt": "nvfp4", "w": torch.zeros(4, 32, dtype=torch.uint8), "sc": torch.zeros(4, 4, dtype=torch.uint8), "s": torch.ones(1), "N": 4, "K": 64}
+    rows = {**one, "fmt": "nvfp4_rows", "s": torch.ones(4)}
+    out = torch.zeros(4, 64)
+    for q, s in ((one, torch.ones(4)), (rows, torch.ones(1))):
+        for bad, word in (({"w": q["w"][:3]}, "w must"), ({"w": torch.zeros(4, 64, dtype=torch.uint8)[:, ::2]}, "w must"), ({"w": torch.zeros(4, 32)}, "w must"),
+                          ({"sc": q["sc"][:3]}, "sc must"), ({"sc": torch.zeros(4, 8, dtype=torch.uint8)[:, ::2]}, "sc must"), ({"s": s}, "s must"),
+                          ({"s": q["s"].double()}, "s must"), ({"N": 5}, "w must"), ({"K": 128}, "w must"), ({"K": 8}, "multiple of 16"), ({}, "CUDA tensors")):
+            with pytest.raises(C.QmoeError, match=word):
+                D.dequant({**q, **bad})
+            if q is rows:
+                with pytest.raises(C.QmoeError, match=word):
+                    D.dequant_rows({**q, **bad}, 0, 4, out)

@@ -383,3 +383,26 @@ def test_gemm_in_one_wave_of_wide_tiles(M, N, K):
         assert torch.equal(D.gemm(q, xq, dtype, act="relu2"), (torch.relu(base.float()) ** 2).to(dtype))
         assert torch.equal(D.gemm(q, xq, dtype, residual=res), (base.float() + res.float()).to(dtype))
     assert D.gemm_status() == 0
+
+
+def test_the_inverse_refuses_what_it_cannot_read():
+    """Scales that stayed on the CPU, outputs of another size; scales in their own type are the same bytes."""
+    import _qmoe_lib as C
+    import dense_q as D
+    x = torch.randn(5, 64, generator=seeded(14), device=DEV)
+    for per_row in (True, False):
+        q = D.quantize(x, per_row)
+        for name in ("w", "sc", "s"):
+            with pytest.raises(C.QmoeError, match="one device"):
+                D.dequant({**q, name: q[name].cpu()})
+        assert torch.equal(D.dequant({**q, "sc": q["sc"].view(torch.float8_e4m3fn)}), D.dequant(q))
+    q = D.quantize(x)
+    for name in ("w", "sc", "s"):
+        with pytest.raises(C.QmoeError, match="one device"):
+            D.dequant_rows({**q, name: q[name].cpu()}, 0, 5, torch.empty(5, 64, device=DEV))
+    for lo, hi, out in ((0, 5, torch.empty(4, 64, device=DEV)), (0, 5, torch.empty(5, 64)), (3, 2, torch.empty(1, 64, device=DEV)),
+                        (3, 6, torch.empty(3, 64, device=DEV)), (-1, 2, torch.empty(3, 64, device=DEV))):
+        with pytest.raises(C.QmoeError):
+            D.dequant_rows(q, lo, hi, out)
+    assert torch.equal(D.dequant_rows(q, 2, 4, torch.empty(2, 64, device=DEV)), values_of(q)[2:4].float())
+    assert D.dequant_rows(q, 2, 2, torch.empty(0, 64, device=DEV)).numel() == 0
