@@ -424,13 +424,22 @@ __device__ __forceinline__ void commit_pair(uint64_t *bar) {
                  "h"((uint16_t)3)
                  : "memory");
 }
-__device__ __forceinline__ void commit_one(uint64_t *bar) {   // on the issuing CTA's barrier alone
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ uint32_t in_leader(const void *p) {   // the same place in the pair's first CTA
     uint32_t r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
     return r;
+}
+
+// A word of the other CTA's shared memory, at this one's place.
+__device__ __forceinline__ void tell(const volatile uint32_t *p, int rank, uint32_t v) {
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\tst.shared::cluster.b32 [r], %2;\n\t}" ::"r"(
+                     smem_u32(const_cast<const uint32_t *>(p))),
+                 "r"(rank), "r"(v)
+                 : "memory");
+}
+// Counts `bytes` as copied on a barrier of this CTA.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 // tmem_ld32 in two halves, so that several loads are in flight; the wait takes the registers, so that none is used before.
@@ -532,6 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t *drain = acc_free + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + P::OFF_MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(sm + P::OFF_MISC + 8);
+    volatile uint32_t *other_loaded = tmem_slot + 1, *other_abort = tmem_slot + 3;   // written by the other CTA
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = blockIdx.x & 1, first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
@@ -546,6 +556,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_init(&acc_free[1], 8);
         mbar_init(drain, 1);
         *abort_flag = 0;
+        *other_loaded = *other_abort = 0;
         fence_mbar_init();
     }
     if (warp == 5) {
@@ -591,6 +602,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             }
         }
+        __syncwarp();
+        if (lane == 0) tell(other_loaded, rank ^ 1, q);
         __syncwarp();
     } else if (warp == 5) {
         // ------------------------------------------------------------ the first CTA's warp drives both tensor cores
@@ -715,20 +728,30 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (*abort_flag && lane == 0) {
-        // As in gemm_kernel; a stage that only one CTA loaded never completes, and its wait ends by its bound, long
-        // after the copies have landed.
-        if (warp == 4 && rank == 0)
-            for (uint32_t u = q > (uint32_t)S ? q - S : 0; u < q; u++) mbar_wait(&full[u % S], (u / S) & 1);
-    }
-    if (warp == 5 && rank == 0 && *abort_flag) {   // the lane that issued: elect picks the same one
-        if (elect_one()) {
-            commit_one(drain);
-            mbar_wait(drain, 0);
-        }
-    }
+    if (tid == 0 && *abort_flag) tell(other_abort, rank ^ 1, 1u);
     __syncwarp();
     cluster_sync();   // neither CTA leaves while the other may still signal it or run on its memory
+    if (*abort_flag || *other_abort) {   // the same in both CTAs
+        // A wait ran out: as in gemm_kernel, what is in flight ends before the pair does. The two CTAs may have given up at
+        // different stages. The first one's barriers count both halves: a stage that only the other loaded is expected
+        // here, the missing half of one that only this CTA loaded counts as copied.
+        if (rank == 0 && warp == 4 && lane == 0) {
+            const uint32_t other = *other_loaded, most = max(q, other);
+            for (uint32_t u = most > (uint32_t)S ? most - S : 0; u < most; u++) {
+                if (u >= q) mbar_expect_tx(&full[u % S], P::BYTES);
+                else if (u >= other) mbar_complete_tx(&full[u % S], P::BYTES);
+                mbar_wait(&full[u % S], (u / S) & 1);
+            }
+        }
+        if (warp == 5) {
+            if (elect_one()) {
+                if (rank == 0) commit_pair(drain);   // the lane that issued: elect picks the same one
+                mbar_wait(drain, 0);
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+    }
     if (warp == 5) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(*tmem_slot) : "memory");

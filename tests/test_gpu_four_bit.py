@@ -406,3 +406,34 @@ def test_the_inverse_refuses_what_it_cannot_read():
             D.dequant_rows(q, lo, hi, out)
     assert torch.equal(D.dequant_rows(q, 2, 4, torch.empty(2, 64, device=DEV)), values_of(q)[2:4].float())
     assert D.dequant_rows(q, 2, 2, torch.empty(0, 64, device=DEV)).numel() == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(100, 4096, 4096), (2000, 4096, 4096), (2048, 2688, 4096), (700, 4097, 2688), (700, 4097, 32768), (2048, 8192, 32768)])
+def test_waits_that_run_out_anywhere_in_a_pair(M, N, K):
+    """Limits from less than one copy's latency to more than the whole product: the two CTAs of a pair give up at stages of
+    their own. Each call either reports it or is right, ends at once (the drain waits for what was issued, not for its
+    2 s bound), and the next one is right. (A single poll of a barrier may outlast a short product: only the long ones
+    surely give up.)"""
+    import time
+
+    import dense_q as D
+    import qmoe_ns as Q
+    g = seeded(M)
+    xq, q = D.prepare(small_integers(g, M, K)), D.prepare(small_integers(g, N, K))
+    ref = D.gemm(q, xq, torch.float32)
+    assert D.gemm_status() == 0
+    late = 0
+    for limit in [1, 1, 100, 300, 600] + list(range(800, 6000, 200)) + list(range(6000, 30000, 2000)):
+        Q.set_wait_cycles(limit)
+        try:
+            torch.cuda.synchronize()
+            start = time.perf_counter()
+            y = D.gemm(q, xq, torch.float32)
+            status = D.gemm_status()
+            assert time.perf_counter() - start < 1.0
+        finally:
+            Q.set_wait_cycles(0)
+        late += status == 4
+        assert status == 4 or (status == 0 and torch.equal(y, ref))
+        assert torch.equal(D.gemm(q, xq, torch.float32), ref) and D.gemm_status() == 0
+    assert late > 0 or K < 32768
