@@ -197,8 +197,9 @@ int qmoe_route_decode(const float *logits, const float *bias, int n_experts, int
 /* Replaces, for any number of tokens, NemotronHMoE.route_tokens_to_experts (tf:697-720) after the router's linear:
  * logits [T, n_experts] in x_dtype, rows ld elements apart. score 0: sigmoid(logit), choice = score + bias [n_experts]
  * (bias may be NULL); 1: the softmax of the row, chosen by the logits (bias NULL). n_group > 1: only the topk_group
- * groups with the largest sums of their two best choices keep them, the others' are 0 (softmax: -inf). ids [T, top_k]
- * the largest choices in decreasing order, ties to the lower id, a NaN last; weights [T, top_k] = score, / (their sum +
+ * groups with the largest sums of their two best choices (softmax: logits) keep them, the others' are 0 (softmax: none,
+ * they are never chosen). ids [T, top_k] the largest choices in decreasing order, ties to the lower id, a NaN as if it
+ * were -inf; weights [T, top_k] = score, / (their sum +
  * 1e-20) when norm != 0, * scaling; counts [n_experts]: tokens that chose each expert. n_experts <= 1024, top_k <= 32,
  * n_group <= 32 groups of at least two, of a softmax the kept ones with at least top_k experts. */
 int qmoe_route(const void *logits, int x_dtype, int64_t ld, const float *bias, int64_t T, int n_experts, int top_k,

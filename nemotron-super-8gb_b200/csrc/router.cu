@@ -2,8 +2,11 @@
 //
 // Routing (decode_step.route_tokens; NemotronHMoE.route_tokens_to_experts, tf:697-720): score = sigmoid(logit) (or the
 // softmax of the row), choice = score + bias, optionally only the best expert groups, the top_k choices in decreasing
-// order (ties to the lower id, a NaN never before a number), weight = score (/ (their sum + 1e-20)) * scaling, and how
-// many tokens chose each expert. Softmax rows are chosen by their logits, which have the same order.
+// order (ties to the lower id, a NaN as if it were -inf), weight = score (/ (their sum + 1e-20)) * scaling, and how
+// many tokens chose each expert. The choice of a softmax row is its logit, which has the scores' order; the sum of a
+// group's two best logits has that of the product of its two best scores (not of their sum). A group that is left out
+// counts as 0 with sigmoids, so that its experts come before negative choices, as the model's router has it; of a
+// softmax none of them is ever chosen.
 //   backward, dw -> dlogits: ds_i = scaling dw_i, or with the sum S over the chosen scaling (dw_i - sum_j dw_j s_j / S) / S;
 //   sigmoid: dl_i = ds_i s_i (1 - s_i) at the chosen; softmax: dl_j = p_j (ds_j - sum_i ds_i p_i) everywhere.
 // Balance loss: p_te = score_te / sum_e score_te, P_e = mean of p_te over the T' unmasked tokens, f_e = E count_e / (k T'),
@@ -178,9 +181,9 @@ __device__ __forceinline__ uint32_t key_of(float c) {
 }
 
 // Keeps the choices of the topk_group groups with the largest sums of their two best choices (ties to the lower group),
-// the others become `fill`. buf: ne floats of this warp.
+// the others become `fill`. buf: ne floats of this warp. Returns which of the lane's choices became so.
 template <int EPL>
-__device__ __forceinline__ void keep_groups(float (&c)[EPL], const Route &a, float fill, float *buf, int lane) {
+__device__ __forceinline__ uint32_t keep_groups(float (&c)[EPL], const Route &a, float fill, float *buf, int lane) {
     const int size = a.ne / a.n_group;
 #pragma unroll
     for (int i = 0; i < EPL; i++)
@@ -208,10 +211,15 @@ __device__ __forceinline__ void keep_groups(float (&c)[EPL], const Route &a, flo
         rank += v > mine || (v == mine && g < lane);
     }
     const uint32_t kept = __ballot_sync(0xffffffffu, lane < a.n_group && rank < a.topk_group);
+    uint32_t out = 0;
 #pragma unroll
     for (int i = 0; i < EPL; i++)
-        if (expert<EPL>(i, lane) < a.ne && !(kept >> (expert<EPL>(i, lane) / size) & 1u)) c[i] = fill;
+        if (expert<EPL>(i, lane) < a.ne && !(kept >> (expert<EPL>(i, lane) / size) & 1u)) {
+            c[i] = fill;
+            out |= 1u << i;
+        }
     __syncwarp();
+    return out;
 }
 
 // The lane's value of a descending bitonic sort of the warp's 32 values.
@@ -234,13 +242,14 @@ struct Candidates {   // of one warp: choice (as a key) and expert, the lower ex
 
 // k rounds of the warp's largest key, of equal ones the lowest expert: lane r gets the r-th. For rows with many equal
 // choices; on random logits of 16384 x 512 these rounds alone took 94 us. FAST: v holds logits, else scores, c choices.
+// Choices in `out` take no part, also where others are -inf (there are k of those).
 template <int EPL, bool FAST>
-__device__ __noinline__ void choose_by_rounds(const Route &a, int lane, const float (&c)[EPL], const float (&v)[EPL], const float *bias, int &id, float &sc) {
+__device__ __noinline__ void choose_by_rounds(const Route &a, int lane, const float (&c)[EPL], const float (&v)[EPL], uint32_t out, const float *bias, int &id, float &sc) {
     uint32_t key[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; i++) {
         const int e = expert<EPL>(i, lane);
-        key[i] = e < a.ne ? key_of(FAST ? fmaxf(sigmoid(v[i]) + bias[e], -INFINITY) : c[i]) : 0u;
+        key[i] = e < a.ne && !(out >> i & 1u) ? key_of(FAST ? fmaxf(sigmoid(v[i]) + bias[e], -INFINITY) : c[i]) : 0u;
     }
     for (int r = 0; r < a.k; r++) {
         uint32_t m = 0;
@@ -277,7 +286,7 @@ __device__ __noinline__ void choose_by_rounds(const Route &a, int lane, const fl
 // the gathered ones alone. With exact scores for all it was 1,580 instructions a token, now 940 (512 experts, ncu):
 // 16384 x 512 in 43, now 25 us.
 template <int EPL, bool FAST>
-__device__ __forceinline__ void choose(const Route &a, int64_t t, int lane, const float (&c)[EPL], const float (&v)[EPL], const float *bias, Candidates &cand, int *hist) {
+__device__ __forceinline__ void choose(const Route &a, int64_t t, int lane, const float (&c)[EPL], const float (&v)[EPL], uint32_t out, const float *bias, Candidates &cand, int *hist) {
     float top = c[0];
 #pragma unroll
     for (int i = 1; i < EPL; i++) top = fmaxf(top, c[i]);
@@ -337,7 +346,7 @@ __device__ __forceinline__ void choose(const Route &a, int64_t t, int lane, cons
         }
         __syncwarp();
     } else {
-        choose_by_rounds<EPL, FAST>(a, lane, c, v, bias, id, sc);
+        choose_by_rounds<EPL, FAST>(a, lane, c, v, out, bias, id, sc);
         if (lane < a.k) rank = lane;
     }
     float total = 1.f;
@@ -395,13 +404,17 @@ template <typename T, int EPL, bool FAST> __global__ void __launch_bounds__(ROUT
                 c[i] = fmaxf(v[i] + bias[expert<EPL>(i, lane)], -INFINITY);      // no score is -0, so no choice is
             }
         }
+        uint32_t out = 0;   // choices that are none
         if constexpr (!FAST)
-            if (a.n_group > 1) keep_groups<EPL>(c, a, a.softmax ? -INFINITY : 0.f, buf, lane);
+            if (a.n_group > 1) {
+                const uint32_t u = keep_groups<EPL>(c, a, a.softmax ? -INFINITY : 0.f, buf, lane);
+                if (a.softmax) out = u;
+            }
         if (a.ne < SLOTS)
 #pragma unroll
             for (int i = 0; i < EPL; i++)
                 if (expert<EPL>(i, lane) >= a.ne) c[i] = -INFINITY;
-        choose<EPL, FAST>(a, t, lane, c, v, bias, cand, hist);
+        choose<EPL, FAST>(a, t, lane, c, v, out, bias, cand, hist);
     }
     if (a.cluster) {
         cluster_sync();

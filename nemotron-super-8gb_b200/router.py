@@ -13,8 +13,10 @@ def route(logits, bias=None, top_k=22, scaling=5.0, n_group=1, topk_group=1, nor
     Score sigmoid(logit), choice score + bias [E] f32; with n_group > 1 only the topk_group groups whose two best
     choices have the largest sum keep theirs (the others' become 0, as the model's router has it); the top_k <= 32
     largest choices; weight = score, divided by the sum of the chosen (+ 1e-20) with norm_topk_prob, times scaling.
-    score "softmax": the softmax over the experts, chosen by the logits, no bias, groups left out entirely (the kept
-    ones need top_k experts). A NaN is chosen last. Differentiable in the logits through the weights."""
+    score "softmax": the softmax over the experts, the choice is the logit, no bias; groups are ranked by the sum of their
+    two best logits (the order of the product of their two best scores, which is not that of the scores' sum or of the
+    best score alone) and left out entirely, so the kept ones need top_k experts, and one of them with a logit of -inf
+    is chosen before any that is left out. A NaN counts as -inf. Differentiable in the logits through the weights."""
     return C.bind().route(logits, bias, top_k, scaling, n_group, topk_group, norm_topk_prob, score)
 
 

@@ -544,3 +544,34 @@ def test_balance_of_batches_beyond_32_tokens_per_warp(T, E, masked):
         error = (got.double() - ref).abs() - TOL * p * (c + dot)
         assert float(error[keep].max()) <= 0 and not got[~keep].any()
         assert bool(got[keep][-1].any())
+
+
+def test_softmax_groups_left_out_are_never_chosen():
+    """Kept groups with fewer finite logits than top_k: their experts at -inf, of the type's lowest value or NaN follow, by
+    value and then by id; the left-out groups' experts do not, however large their softmax weight. The reference sorts
+    (kept, value) pairs."""
+    import router as R
+    g = seeded(91)
+    for E, n_group, kept, k in ((32, 4, 2, 12), (96, 8, 3, 32), (512, 8, 4, 22), (1024, 32, 2, 32), (160, 8, 1, 20)):
+        size = E // n_group
+        x = torch.randn(40, n_group, size, generator=g, device=DEV)
+        strong = torch.argsort(torch.rand(40, n_group, generator=g, device=DEV), dim=1)[:, :kept]    # the groups to keep
+        keep = torch.zeros(40, n_group, dtype=torch.bool, device=DEV).scatter_(1, strong, True)
+        x[..., :2] += 30.0 * keep[..., None]
+        x[..., 2:] = torch.where(keep[..., None] & (torch.rand(x[..., 2:].shape, generator=g, device=DEV) < 0.95), -float("inf"), x[..., 2:])
+        x[5:10, :, size - 1] = torch.where(keep[5:10], torch.finfo(torch.float32).min, x[5:10, :, size - 1])
+        x[10:15] = torch.where(keep[10:15, :, None] & (x[10:15] == -float("inf")) & (torch.arange(size, device=DEV) % 2 == 0), float("nan"), x[10:15])
+        x[20, :, 1:] = -float("inf")                       # no group has a sum: the first ones are kept
+        keep[20] = torch.arange(n_group, device=DEV) < kept
+        flat, on = x.reshape(40, E), keep.repeat_interleave(size, 1)
+        value = torch.where(torch.isnan(flat), -float("inf"), flat)
+        by_value = torch.sort(value, dim=1, descending=True, stable=True)[1]
+        first = torch.sort(on.gather(1, by_value).to(torch.int8), dim=1, descending=True, stable=True)[1]
+        want = by_value.gather(1, first)[:, :k]
+        leaf = flat.clone().requires_grad_()
+        ids, w, n = R.route(leaf, None, top_k=k, n_group=n_group, topk_group=kept, score="softmax")
+        assert bool(on.gather(1, ids).all()) and torch.equal(ids, want)
+        assert torch.equal(n, torch.bincount(ids.flatten(), minlength=E).to(torch.int32))
+        ref = weights64(flat.double(), ids, 5.0, False, "softmax")
+        assert torch.allclose(w.detach().double(), ref, rtol=TOL, atol=5e-30, equal_nan=True)
+        assert not w.detach()[:5][flat[:5].gather(1, ids[:5]) == -float("inf")].any()
