@@ -81,7 +81,11 @@ template <typename T = void> T *data(const OptTensor &t) { return t.has_value() 
 template <typename T = void> T *data(const Tensor &t) { return static_cast<T *>(t.data_ptr()); }
 
 // ------------------------------------------------------------------------------------------ four bits
+// A forward-mode tangent, which torch carries on under no_grad too, would be lost.
+void no_tangent(const Tensor &t, const char *who) { REQUIRE(!torch::autograd::isFwGradDefined(t), who, " operators have no forward-mode derivative"); }
+
 void no_grad(const Tensor &t) {
+    no_tangent(t, "the four-bit");
     REQUIRE(!(t.requires_grad() && at::GradMode::is_enabled()), "the four-bit operators have no gradient: call them under torch.no_grad()");
 }
 
@@ -294,9 +298,8 @@ struct Gradient : torch::autograd::Node {
 void attach(const Tensor &out, std::shared_ptr<torch::autograd::Node> node) { torch::autograd::set_history(out, node); }
 
 bool differentiated(const Tensor &x) {
-    if (!at::GradMode::is_enabled()) return false;
-    REQUIRE(!torch::autograd::isFwGradDefined(x), "the router's operators have no forward-mode derivative");
-    return x.requires_grad();
+    no_tangent(x, "the router's");
+    return at::GradMode::is_enabled() && x.requires_grad();
 }
 
 struct RouteBackward : Gradient {

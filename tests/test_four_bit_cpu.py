@@ -165,3 +165,19 @@ def test_the_inverse_looks_at_its_tensors():
             if q is rows:
                 with pytest.raises(C.QmoeError, match=word):
                     D.dequant_rows({**q, **bad}, 0, 4, out)
+
+
+def test_forward_mode_tangents_are_refused():
+    """They are carried on under no_grad as well, so that a result without one would be silently wrong."""
+    import _qmoe_lib as C
+    import dense_q as D
+    import torch.autograd.forward_ad as fwd
+    rows = {"fmt": "nvfp4_rows", "w": torch.zeros(2, 32, dtype=torch.uint8), "sc": torch.zeros(2, 4, dtype=torch.uint8),
+            "s": torch.ones(2), "N": 2, "K": 64}
+    x = torch.zeros(2, 64)
+    for grad in (True, False):
+        with fwd.dual_level(), torch.set_grad_enabled(grad):
+            dual, res = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(torch.zeros(2, 2, dtype=torch.bfloat16), torch.ones(2, 2, dtype=torch.bfloat16))
+            for bad in (lambda: D.quantize(dual), lambda: D.qlinear_a4(rows, dual), lambda: D.gemm(rows, rows, residual=res)):
+                with pytest.raises(C.QmoeError, match="forward-mode"):
+                    bad()

@@ -575,3 +575,18 @@ def test_softmax_groups_left_out_are_never_chosen():
         ref = weights64(flat.double(), ids, 5.0, False, "softmax")
         assert torch.allclose(w.detach().double(), ref, rtol=TOL, atol=5e-30, equal_nan=True)
         assert not w.detach()[:5][flat[:5].gather(1, ids[:5]) == -float("inf")].any()
+
+
+def test_forward_mode_tangents_are_refused_without_grad_mode_too():
+    import _qmoe_lib as C
+    import router as R
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(6, 32, generator=seeded(92), device=DEV)
+    ids = torch.topk(x, 3)[1]
+    for grad in (True, False):
+        with fwd.dual_level(), torch.set_grad_enabled(grad):
+            dual = fwd.make_dual(x, torch.ones_like(x))
+            for bad in (lambda: R.route(dual, None, top_k=3), lambda: R.balance_loss(dual, ids)):
+                with pytest.raises(C.QmoeError, match="forward-mode"):
+                    bad()
+            assert not R.route(x, None, top_k=3)[1].requires_grad and not R.balance_loss(x, ids)[0].requires_grad
