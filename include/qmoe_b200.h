@@ -332,8 +332,8 @@ int dq_gemm_nvfp4(const uint8_t *w, const uint8_t *w_atoms, const float *sw, int
 /* dq_quantize_nvfp4 (per row) and dq_gemm_nvfp4 in one call: y [M, N] in x_dtype from x [M, K], rows ldx elements apart,
  * and a weight given with its scales both as stored (w_sc [N, K/16]) and as atoms. Up to four rows run as one kernel that
  * quantizes and multiplies (the sums then run in another order). The workspace (16-byte aligned;
- * dq_linear_a4_workspace_bytes(M, K), 0 for sizes out of range; not looked at, so possibly NULL, for M <= 4 with
- * K <= 16384) holds the quantized rows and needs no initial value; it must not be used by another call running
+ * dq_linear_a4_workspace_bytes(M, K), 0 for sizes out of range; like the atoms not looked at, so possibly NULL, for M <= 4
+ * with K <= 16384) holds the quantized rows and needs no initial value; it must not be used by another call running
  * concurrently. */
 size_t dq_linear_a4_workspace_bytes(int64_t M, int64_t K);
 int dq_linear_a4(const uint8_t *w, const uint8_t *w_sc, const uint8_t *w_atoms, const float *sw, int sw_per_row, const void *x,

@@ -220,10 +220,13 @@ Tensor linear_a4(const Tensor &w, const Tensor &sc, OptTensor atoms, const Tenso
     const Tensor y = empty(shape, x, x.scalar_type());
     if (M && N) {
         REQUIRE(M <= (1 << 24), "gemm: at most 2^24 rows");
-        if (!atoms) atoms = scale_atoms(w, sc, s, w_rows, N, K);
         OptTensor ws;
-        const size_t n = M > 4 || K > 16384 ? dq_linear_a4_workspace_bytes(M, K) : 0;   // few rows need none
-        if (n) ws = empty({(int64_t)n}, x, at::kByte);
+        size_t n = 0;
+        if (M > 4 || K > 16384) {   // few rows need neither
+            if (!atoms) atoms = scale_atoms(w, sc, s, w_rows, N, K);
+            n = dq_linear_a4_workspace_bytes(M, K);
+            ws = empty({(int64_t)n}, x, at::kByte);
+        }
         status(dq_linear_a4(data<uint8_t>(w), data<uint8_t>(sc), data<uint8_t>(atoms), data<float>(s), w_rows, data(x), dt, ld, (int)M, (int)N, (int)K, ep,
                             data(residual), data(y), data(ws), n, stream_of(x)), "dq_linear_a4");
     }

@@ -200,7 +200,7 @@ int dq_linear_a4(const uint8_t *w, const uint8_t *w_sc, const uint8_t *w_atoms, 
                  int x_dtype, int64_t ldx, int M, int N, int K, int epilogue, const void *residual, void *y, void *workspace,
                  size_t workspace_bytes, void *stream) {
     const bool few = M <= g4::TOKENS && K <= 16384;   // up to 128 KB of quantised rows in shared memory
-    if (!w || !w_sc || !w_atoms || !sw || !x || !y || (!workspace && !few) || (epilogue == 2 && !residual)) return QMOE_ERR_NULL;
+    if (!w || !w_sc || !sw || !x || !y || (!few && (!w_atoms || !workspace)) || (epilogue == 2 && !residual)) return QMOE_ERR_NULL;
     const size_t need = dq_linear_a4_workspace_bytes(M, K);
     if (!need || N < 1 || N > (1 << 24) || epilogue < 0 || epilogue > 2 || ldx < K) return QMOE_ERR_SHAPE;
     if (!valid_dtype(x_dtype)) return QMOE_ERR_DTYPE;

@@ -181,3 +181,13 @@ def test_forward_mode_tangents_are_refused():
             for bad in (lambda: D.quantize(dual), lambda: D.qlinear_a4(rows, dual), lambda: D.gemm(rows, rows, residual=res)):
                 with pytest.raises(C.QmoeError, match="forward-mode"):
                     bad()
+
+
+def test_few_rows_need_no_scale_atoms(lib):
+    a = P(256)
+    need = lib.dq_linear_a4_workspace_bytes(5, 64)
+
+    def call(atoms, M):
+        return lib.dq_linear_a4(a, a, atoms, a, 0, a, 1, 64, M, 8, 64, 0, None, a, a, need, None)
+
+    assert call(None, 5) == 5 and call(None, 4) != 5

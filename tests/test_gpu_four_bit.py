@@ -437,3 +437,17 @@ def test_waits_that_run_out_anywhere_in_a_pair(M, N, K):
         assert status == 4 or (status == 0 and torch.equal(y, ref))
         assert torch.equal(D.gemm(q, xq, torch.float32), ref) and D.gemm_status() == 0
     assert late > 0 or K < 32768
+
+
+@pytest.mark.parametrize("M", [1, 4, 5])
+def test_linear_of_a_weight_that_was_not_prepared(M):
+    """The same bits as with its scales laid out; few rows take one kernel and lay out nothing."""
+    import dense_q as D
+    g = seeded(M)
+    q = D.quantize(torch.randn(300, 512, generator=g, device=DEV), False)
+    x = torch.randn(M, 512, generator=g, device=DEV).to(torch.bfloat16)
+    want = D.qlinear_a4(D.prepare(q), x)
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    y = D.qlinear_a4(q, x)
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == (1 if M < 5 else 3)   # y; scales, workspace
+    assert torch.equal(y, want)
