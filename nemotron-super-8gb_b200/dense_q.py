@@ -163,11 +163,10 @@ def _nvfp4(q):
 
 
 def prepare(q):
-    """A weight ready for gemm: the dict with "sca", its block scales as the tensor cores read them, added (the
-    other tensors are shared with q)."""
+    """A weight ready for gemm: the dict with "sca", its block scales as the tensor cores read them now, added (the
+    other tensors are shared with q). "sca" is a copy: it does not follow "sc". Products read it instead of "sc" (a linear
+    of up to MB_MAX rows reads "sc"), so a dict whose scales were changed or of which rows were taken is prepared anew."""
     _nvfp4(q)
-    if "sca" in q:
-        return q
     return {**q, "sca": C.bind().scale_atoms(q["w"], q["sc"], q["s"], q["fmt"] == "nvfp4_rows", q["N"], q["K"])}
 
 

@@ -451,3 +451,19 @@ def test_linear_of_a_weight_that_was_not_prepared(M):
     y = D.qlinear_a4(q, x)
     assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == (1 if M < 5 else 3)   # y; scales, workspace
     assert torch.equal(y, want)
+
+
+def test_a_weight_that_changed_is_prepared_anew():
+    """prepare lays out the scales that the dict holds now, an older "sca" or not: few and many rows then agree."""
+    import dense_q as D
+    g = seeded(15)
+    q = D.prepare(small_integers(g, 200, 512))
+    x = torch.randint(-2, 3, (5, 512), generator=g, device=DEV).float()
+    part = {**q, "w": q["w"][40:100].clone(), "sc": q["sc"][40:100].clone(), "N": 60}
+    q["sc"][:, 3] = 0x40
+    for w in (D.prepare(part), D.prepare(q)):
+        fresh = {k: v for k, v in w.items() if k != "sca"}
+        xq = D.quantize(x)
+        want = (values_of(xq) @ values_of(w).t()).float()
+        assert torch.equal(D.qlinear_a4(w, x), want) and torch.equal(D.qlinear_a4(fresh, x), want)
+        assert torch.equal(D.qlinear_a4(w, x[:4]), want[:4]) and torch.equal(D.gemm(w, xq, torch.float32), want)
