@@ -6,9 +6,11 @@ Each csrc/*.cu is compiled to an object in _build/ (in parallel), then linked in
 against the shared CUDA runtime: inside a torch process the library binds to the libcudart.so.12 torch
 already loaded, so both see the same current device and streams; standalone it finds the toolkit's
 runtime through its rpath. csrc/bind.cpp (g++, torch's headers) becomes qmoe_torch.so beside it: the operators that
-are called as functions of torch tensors, over the library's C entry points.
+are called as functions of torch tensors, over the library's C entry points. Where torch is not installed, the library
+alone is built.
 """
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -62,21 +64,24 @@ def build(verbose=False, extra=()):
             raise RuntimeError("nvcc failed: " + " ".join(cmd))
         return r.stdout + r.stderr
 
-    import torch
-    from torch.utils import cpp_extension as T
-    bind_src, bind_obj = os.path.join(CSRC, "bind.cpp"), os.path.join(BUILD, "bind.o")
-    if _stale(bind_obj, [bind_src, headers[-1], torch.version.__file__]):
-        inc = [*T.include_paths("cuda"), sysconfig.get_paths()["include"]]
-        jobs.append(["g++", "-O2", "-std=c++17", "-fPIC", *(f"-I{d}" for d in inc), "-c", bind_src, "-o", bind_obj])
+    library_stale = bool(jobs) or not os.path.exists(LIB)
+    bindings = importlib.util.find_spec("torch") is not None
+    if bindings:
+        import torch
+        from torch.utils import cpp_extension as T
+        bind_src, bind_obj = os.path.join(CSRC, "bind.cpp"), os.path.join(BUILD, "bind.o")
+        if _stale(bind_obj, [bind_src, headers[-1], torch.version.__file__]):
+            inc = [*T.include_paths("cuda"), sysconfig.get_paths()["include"]]
+            jobs.append(["g++", "-O2", "-std=c++17", "-fPIC", *(f"-I{d}" for d in inc), "-c", bind_src, "-o", bind_obj])
     with cf.ThreadPoolExecutor(max(1, min(len(jobs), os.cpu_count() or 4))) as ex:
         logs = list(ex.map(run, jobs))
     objs = [os.path.join(BUILD, os.path.basename(s)[:-3] + ".o") for s in sources()]
-    if jobs or not os.path.exists(LIB):
+    if library_stale:
         tmp = LIB + ".tmp"
         run([nv, *ARCH, "-shared", "-o", tmp, *objs, "-cudart", "shared",
              "-Xlinker", "-rpath=/usr/local/cuda/lib64"])
         os.replace(tmp, LIB)
-    if _stale(BIND, [bind_obj]):
+    if bindings and _stale(BIND, [bind_obj]):
         tmp = BIND + ".tmp"
         run(["g++", "-shared", "-o", tmp, bind_obj, f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", f"-L{HERE}",
              "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lqmoe_b200", "-Wl,-rpath,$ORIGIN"])
