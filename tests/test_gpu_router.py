@@ -590,3 +590,38 @@ def test_forward_mode_tangents_are_refused_without_grad_mode_too():
                 with pytest.raises(C.QmoeError, match="forward-mode"):
                     bad()
             assert not R.route(x, None, top_k=3)[1].requires_grad and not R.balance_loss(x, ids)[0].requires_grad
+
+
+@pytest.mark.parametrize("k", [1, 22, 32])
+@pytest.mark.parametrize("E", [96, 512])
+def test_route_weights_of_ties_and_strange_numbers(E, k):
+    """Saturated, tied, infinite, signed-zero and NaN rows: the weights are torch's own bits at the chosen experts (a NaN
+    where torch has one), and a softmax's are those of 64 bits, NaN for rows that have none. Scores below fp32's normal
+    numbers, 1.2e-38, may be 0: over the sum's 1e-20 and times 5 that is 6e-18 of a weight."""
+    import router as R
+    g = seeded(E)
+    x = torch.randn(16, E, generator=g, device=DEV)
+    x[0] = 0.0
+    x[1, 40:] = 1.0
+    x[2], x[3] = -200.0, 200.0
+    x[4, ::2] = -float("inf")
+    x[5, 10], x[5, 90] = float("inf"), -float("inf")
+    x[6, 3:60] = float("nan")
+    x[7] = torch.arange(E, device=DEV) % 3
+    x[8], x[8, 50:] = -0.0, 0.0
+    x[9] = float("nan")
+    x[10] = -torch.arange(E, device=DEV).float()
+    x[11] = 20.0 + torch.arange(E, device=DEV) % 96 * 0.1
+    x[12, 5:] = -float("inf")
+    x[13, 5:] = torch.finfo(torch.float32).min
+    x[14] = -float("inf")
+    for norm in (False, True):
+        for bias in (None, torch.linspace(-1, 1, E, device=DEV)):
+            ids, w, n = R.route(x, bias, top_k=k)
+            assert torch.equal(ids, chosen(x, bias, k))
+            assert torch.equal(torch.nan_to_num(w, nan=-1.0), torch.nan_to_num(torch.sigmoid(x).gather(1, ids) * 5.0, nan=-1.0))
+            ids, w, _ = R.route(x, bias, top_k=k, norm_topk_prob=True)
+            assert torch.allclose(w.double(), weights64(x.double(), ids, 5.0, True, "sigmoid"), rtol=TOL, atol=5e-17, equal_nan=True)
+        ids, w, n = R.route(x, None, top_k=k, score="softmax", norm_topk_prob=norm)
+        assert torch.equal(ids, chosen(x, None, k, score="softmax"))
+        assert torch.allclose(w.double(), weights64(x.double(), ids, 5.0, norm, "softmax"), rtol=TOL, atol=5e-17 if norm else 5e-30, equal_nan=True)
