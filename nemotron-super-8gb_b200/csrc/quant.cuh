@@ -4,9 +4,9 @@
 //   s  = 2^e, the smallest power of two >= 2^-126 with amax <= 6 * 448 * s,
 //   sc = e4m3(amax16 / (6 s)), nearest, ties to even,
 //   q  = e2m1(x / (s sc)), nearest, ties to even; value = q * sc * s.
-// A power of two loses nothing against s = amax / 2688: the block scale is itself a floating-point number, and
-// x / s is then exact. A block that holds an infinity or a NaN gets the scale NaN (0x7F) and zero codes; s ignores
-// those elements.
+// Against s = amax / 2688 a power of two costs up to one binade at the lower end of the block scales' range, and nothing
+// above it: the block scale is itself a floating-point number. x / s is exact. A block that holds an infinity or a NaN
+// gets the scale NaN (0x7F) and zero codes; s ignores those elements.
 //
 // Every decision is the exact one, without a division. What is compared is x / s with midpoint * sc, or amax16 / s with
 // 6 * midpoint: numbers of at most 7 significant bits. An fp32 x is first cut to 13 bits with the rest ORed into the last

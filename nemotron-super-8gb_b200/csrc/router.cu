@@ -14,8 +14,9 @@
 //
 // All four kernels give a token to a warp, which holds its logits in registers, one per lane and 32 experts: the row is
 // read once and every sum over experts is a warp's. The loss's gradient runs near the logits' bytes (32768 x 512 fp32 with
-// a fifth masked: 121 MB in 21 us); its sums (54 MB in 20 us) and the routing (16384 x 512: 34 MB in 25 us) are bound by
-// issue, by the sigmoid and the selection.
+// a fifth masked: 121 MB in 21 us). Its sums (54 MB in 20 us) and the routing (16384 x 512: 34 MB in 25 us) take twice the
+// time of their instructions at the full issue rate (9 and 13 us): a token's load and its chains of shuffles, with eight
+// warps per scheduler and nothing of the next token in flight, are the rest.
 #include <cmath>
 
 #include "common.cuh"
@@ -508,7 +509,8 @@ template <int EPL> constexpr int BAL_WARPS = EPL > 16 ? 16 : 32;
 
 // sigmoid and 1 - sigmoid as products of one reciprocal (1 ulp), where nothing is decided by their last bit, as it is in
 // the routing: neither loses digits near 1. e^-x is 2^y for y = fl(-x log2 e), corrected by what that rounding left.
-// x is kept to [-87, 126] (a NaN stays one), where all of it is a normal number; what lies outside counts as the border.
+// x is kept to [-87, 126] (a NaN stays one), where no step overflows; what lies outside counts as the border. From 87.3 on
+// e^-x lies below the normal numbers and is 0, and 1 - sigmoid with it.
 __device__ __forceinline__ void sigmoid_pair(float x, float &s, float &r) {
     asm("max.NaN.f32 %0, %0, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42FC0000;" : "+f"(x));
     constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;

@@ -47,7 +47,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
 
-// 3-D tiled TMA load (box {x, y, 1}) into this CTA's shared memory, completing on `bar`.
 // 1-D bulk copy global -> shared (16-byte aligned addresses, size a multiple of 16), completing on bar.
 __device__ __forceinline__ void bulk_g2s_nohint(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -56,6 +55,7 @@ __device__ __forceinline__ void bulk_g2s_nohint(void *dst, const void *src, uint
                  : "memory");
 }
 
+// 3-D tiled TMA load (box {x, y, 1}) into this CTA's shared memory, completing on `bar`.
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
@@ -64,7 +64,6 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, i
         : "memory");
 }
 
-// 32 lanes x 16 consecutive f32 columns of tensor memory -> 16 registers per thread.
 // 16 consecutive 32-bit columns of this warp's 32 TMEM lanes from registers (thread i -> lane base + i).
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
